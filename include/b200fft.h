@@ -447,6 +447,119 @@ void b200fft_ticket_destroy(b200fft_ticket *ticket);
  * NativeRuntime, clearing it. */
 b200fft_status b200fft_context_synchronize(b200fft_context *context, void *stream);
 
+/* ---- sequence operators ---------------------------------------------------
+ * Layer normalisation and linear attention with a decay per head: the operators of a
+ * sequence-mixing block that stand beside the FFT convolution (whose filter is fixed; the
+ * attention's depends on the data).  No counterpart in the reference.  Device pointers,
+ * stream ordered; building and validating a configuration touches no GPU.
+ * As for b200fft_execute, a NULL stream is the context's own; to run on CUDA's legacy
+ * default stream pass cudaStreamLegacy, (void *)1.  Optional pointers may be NULL.
+ * Pointers must be aligned to their elements (state and statistics: 4 bytes, offsets: 8);
+ * outputs must not overlap inputs unless said so.  Kernels take wider accesses where
+ * addresses and strides allow them, and the results do not depend on that. */
+typedef enum b200fft_element_type {
+    B200FFT_ELEMENT_F32 = 0,
+    B200FFT_ELEMENT_F16 = 1,
+    B200FFT_ELEMENT_BF16 = 2
+} b200fft_element_type;
+
+/* y = (x - mean) * rstd * weight + bias over the last axis of [rows, features], with
+ * rstd = 1 / sqrt(variance + epsilon); statistics and sums in 32 bits. */
+typedef struct b200fft_layer_norm_config {
+    uint64_t rows, features;
+    uint64_t input_row_stride;  /* elements between rows of x and dx; 0: features */
+    uint64_t output_row_stride; /* of y and dy; 0: features */
+    float epsilon;              /* >= 0; b200fft_layer_norm_config_init sets 1e-5 */
+    int32_t element_type;       /* x, y, dx, dy: b200fft_element_type */
+    int32_t parameter_type;     /* weight, bias and their gradients */
+    int32_t _reserved;
+} b200fft_layer_norm_config;
+typedef struct b200fft_layer_norm b200fft_layer_norm;
+
+b200fft_status b200fft_layer_norm_config_init(b200fft_layer_norm_config *config, uint64_t rows, uint64_t features);
+b200fft_status b200fft_layer_norm_config_validate(const b200fft_layer_norm_config *config);
+b200fft_status b200fft_layer_norm_build(const b200fft_layer_norm_config *config, const b200fft_device_profile *device,
+                                        b200fft_layer_norm **layer_norm);
+void b200fft_layer_norm_destroy(b200fft_layer_norm *layer_norm);
+/* Device scratch of the backward pass (the forward pass needs none). */
+uint64_t b200fft_layer_norm_backward_workspace_bytes(const b200fft_layer_norm *layer_norm);
+/* weight NULL: ones; bias NULL: zeros; mean and rstd (f32, one per row) are written where
+ * given.  output may be the input itself (same address and stride). */
+b200fft_status b200fft_execute_layer_norm(b200fft_context *context, b200fft_layer_norm *layer_norm, const void *input,
+                                          const void *weight, const void *bias, void *output, float *mean, float *rstd,
+                                          void *stream);
+/* mean and rstd as the forward pass left them.  Each gradient is written where given;
+ * weight NULL: ones.  The weight's and the bias's gradients are sums over the rows in a
+ * fixed order (equal inputs give equal bits).  input_gradient may be output_gradient.
+ * workspace NULL: context-owned scratch. */
+b200fft_status b200fft_execute_layer_norm_backward(b200fft_context *context, b200fft_layer_norm *layer_norm,
+                                                   const void *input, const void *weight, const float *mean,
+                                                   const float *rstd, const void *output_gradient,
+                                                   void *input_gradient, void *weight_gradient, void *bias_gradient,
+                                                   void *workspace, void *stream);
+
+/* Per head h with l = exp(log_decay[h]):  S_t = l S_(t-1) + k_t v_t^T  (key_dim x value_dim,
+ * f32),  o_t = scale * S_t^T q_t.  Tensors are [batch, token, head, dim] with the last axis
+ * contiguous; heads / key_value_heads query heads share one key/value head. */
+typedef struct b200fft_linear_attention_config {
+    uint64_t batch_count;     /* sequences */
+    uint64_t length;          /* tokens of each sequence; packed: of the longest */
+    uint64_t heads;           /* query and output heads */
+    uint64_t key_value_heads; /* a divisor of heads */
+    uint64_t key_dim, value_dim;
+    int32_t packed;           /* 1: sequences stand behind one another in packed_tokens rows */
+    int32_t element_type;     /* q, k, v, o and their gradients */
+    uint64_t packed_tokens;
+    uint64_t state_slots;     /* states in the state buffers; 0: batch_count */
+    float scale;              /* b200fft_linear_attention_config_init sets 1 / sqrt(key_dim) */
+    int32_t _reserved;
+    /* elements between batches (unused when packed), tokens and heads; 0: dense */
+    uint64_t query_strides[3], key_strides[3], value_strides[3], output_strides[3];
+} b200fft_linear_attention_config;
+typedef struct b200fft_linear_attention b200fft_linear_attention;
+
+b200fft_status b200fft_linear_attention_config_init(b200fft_linear_attention_config *config, uint64_t length,
+                                                    uint64_t heads, uint64_t key_dim, uint64_t value_dim);
+b200fft_status b200fft_linear_attention_config_validate(const b200fft_linear_attention_config *config);
+b200fft_status b200fft_linear_attention_build(const b200fft_linear_attention_config *config,
+                                              const b200fft_device_profile *device,
+                                              b200fft_linear_attention **attention);
+void b200fft_linear_attention_destroy(b200fft_linear_attention *attention);
+uint64_t b200fft_linear_attention_workspace_bytes(const b200fft_linear_attention *attention);
+uint64_t b200fft_linear_attention_backward_workspace_bytes(const b200fft_linear_attention *attention);
+
+typedef struct b200fft_linear_attention_buffers {
+    const void *query, *key, *value;
+    const float *log_decay;           /* [heads], <= 0; -infinity forgets everything before the token */
+    const int64_t *sequence_offsets;  /* packed: [batch_count + 1], rows of sequence b: [o[b], o[b+1]);
+                                       * rows outside the buffers or beyond `length` are left out */
+    const int32_t *state_slots;       /* [batch_count], slot of each sequence; NULL: b.  A slot outside
+                                       * [0, state_slots): starts from zero, its state is not kept */
+    const float *initial_state;       /* [state_slots, heads, key_dim, value_dim]; NULL: zeros */
+    void *output;
+    float *final_state;               /* NULL: not kept; may be initial_state itself */
+} b200fft_linear_attention_buffers;
+/* Whole sequences, or (length 1) one new token of each: continue from initial_state. */
+b200fft_status b200fft_execute_linear_attention(b200fft_context *context, b200fft_linear_attention *attention,
+                                                const b200fft_linear_attention_buffers *buffers, void *workspace,
+                                                void *stream);
+
+typedef struct b200fft_linear_attention_gradients {
+    const void *query, *key, *value;
+    const float *log_decay;
+    const int64_t *sequence_offsets;
+    const float *initial_state;         /* [batch_count, heads, key_dim, value_dim], as all states here; NULL: zeros */
+    const void *output_gradient;        /* strides of the output */
+    const float *final_state_gradient;  /* NULL: zeros */
+    void *query_gradient, *key_gradient, *value_gradient; /* strides of their tensors; NULL: not wanted */
+    float *initial_state_gradient;      /* NULL: not wanted; may be final_state_gradient itself */
+} b200fft_linear_attention_gradients;
+/* Gradients of shared key/value heads are sums over their query heads, in a fixed order.
+ * The decay is a constant of the head and has no gradient. */
+b200fft_status b200fft_execute_linear_attention_backward(b200fft_context *context, b200fft_linear_attention *attention,
+                                                         const b200fft_linear_attention_gradients *gradients,
+                                                         void *workspace, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

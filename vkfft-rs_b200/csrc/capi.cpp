@@ -5,6 +5,7 @@
 #include <memory>
 
 #include "aot.hpp"
+#include "capi_guard.hpp"
 #include "runtime.hpp"
 #include "slab.hpp"
 
@@ -15,9 +16,6 @@ struct b200fft_plan {
 };
 struct b200fft_transform {
     std::unique_ptr<Transform> t;
-};
-struct b200fft_context {
-    Context *ctx;
 };
 struct b200fft_convolution {
     std::unique_ptr<Convolution> c;
@@ -31,26 +29,7 @@ struct b200fft_ticket {
 
 static thread_local std::string g_last_error;
 
-template <typename F>
-static b200fft_status guarded(F &&f) {
-    try {
-        f();
-        return B200FFT_OK;
-    } catch (const FftError &e) {
-        g_last_error = e.message;
-        return e.code;
-    } catch (const std::bad_alloc &) {
-        g_last_error = "CUDA runtime error: host allocation failed";
-        return B200FFT_NATIVE_RUNTIME;
-    } catch (const std::exception &e) {
-        g_last_error = std::string("CUDA runtime error: ") + e.what();
-        return B200FFT_NATIVE_RUNTIME;
-    }
-}
-
-static void need(const void *p, const char *what) {
-    if (!p) throw FftError(B200FFT_VALUE_OUT_OF_RANGE, std::string(what) + " must not be null");
-}
+void b200fft::set_last_error(std::string message) { g_last_error = std::move(message); }
 
 static DeviceProfile profile_from_c(const b200fft_device_profile &c) {
     DeviceProfile d;

@@ -187,6 +187,14 @@ static void *ensure_buffer(void *&buf, size_t &have, size_t need, const char *wh
     return buf;
 }
 
+void *context_scratch(Context *ctx, size_t bytes) {
+    return ensure_buffer(ctx->scratch, ctx->scratch_bytes, bytes, "scratch allocation");
+}
+
+void before_launch() {
+    if (injected("launch", g_launch_count)) fail_runtime("kernel launch failed: injected launch fault");
+}
+
 void execute_program(Context *ctx, uint64_t id, const Program &prog, const void *in, void *out, void *workspace,
                      cudaStream_t stream, const PeerStore *peer, cudaEvent_t before_last) {
     check(cudaSetDevice(ctx->device), "cudaSetDevice");
@@ -242,7 +250,7 @@ void execute_program(Context *ctx, uint64_t id, const Program &prog, const void 
                 rp.peer = *peer;
                 rp.peer.sub = peer->chunk * pp.peer_es;
             }
-            if (injected("launch", g_launch_count)) fail_runtime("kernel launch failed: injected launch fault");
+            before_launch();
             check(launch_reg(rv, rp, stream), "kernel launch");
             continue;
         }
@@ -260,7 +268,7 @@ void execute_program(Context *ctx, uint64_t id, const Program &prog, const void 
             p.peer = *peer;
             p.peer.sub = peer->chunk * pp.peer_es;
         }
-        if (injected("launch", g_launch_count)) fail_runtime("kernel launch failed: injected launch fault");
+        before_launch();
         if (pi < dt.spec.size() && dt.spec[pi]) {
             void *args[] = {&p};
             check(cudaLaunchKernel(dt.spec[pi], dim3((unsigned)pp.grid), dim3(pp.threads), args, pp.smem, stream),
@@ -327,7 +335,8 @@ void execute_program_host(Context *ctx, uint64_t id, const Program &prog, const 
 static std::string describe_error_word(int err) {
     std::string m = "B200 FFT kernel reported error word " + std::to_string(err);
     if (err & 32) m += " (slab exchange barrier timed out: a peer rank did not arrive)";
-    if (err & ~32) m += " (invalid pass program)";
+    if (err & 64) m += " (linear attention: a wait for the tensor cores or a copy expired)";
+    if (err & ~(32 | 64)) m += " (invalid pass program)";
     return m;
 }
 

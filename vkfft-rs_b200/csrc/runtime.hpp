@@ -60,6 +60,11 @@ Context *context_create(int device);
 void context_destroy(Context *ctx);
 void forget_program(uint64_t id);  // drop uploaded tables of a destroyed transform from every context
 
+// The context's growable scratch arena (the caller holds ctx->mu).
+void *context_scratch(Context *ctx, size_t bytes);
+// Host-side fault injection: fails the launch that B200FFT_FAULT names.
+void before_launch();
+
 // Stream-ordered execution of a program on device pointers.  peer: the exchange
 // buffers of the ranks for passes marked peer_scatter (slab transforms only).
 // before_last: an event recorded on the stream just before the last pass is launched

@@ -1,0 +1,58 @@
+// Element conversions and the row ranges that the sequence kernels share.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "sequence.hpp"
+
+namespace b200fft {
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int m = 16; m; m >>= 1) v += __shfl_xor_sync(~0u, v, m);
+    return v;
+}
+
+// First row and number of rows of sequence b.  Offsets are data: whatever they hold, the
+// range stays inside the packed rows and no longer than `length`.
+struct Rows {
+    int64_t start;
+    int64_t count;
+};
+__device__ __forceinline__ Rows rows_of(const int64_t *offsets, int64_t packed_tokens, int64_t length, int64_t b) {
+    if (!offsets) return {0, length};
+    const int64_t total = packed_tokens;
+    const int64_t a = min(max(offsets[b], (int64_t)0), total);
+    const int64_t e = min(max(offsets[b + 1], a), total);
+    return {a, min(e - a, length)};
+}
+
+// l^n of a head, n >= 0.  n = 0 is 1 even where the logarithm is -infinity.
+__device__ __forceinline__ float decay_power(float log_decay, float n) {
+    return n > 0.f ? expf(log_decay * n) : 1.f;
+}
+
+// Calls f with a value of the element's type.
+template <typename F>
+cudaError_t with_element(Element e, F &&f) {
+    switch (e) {
+        case Element::F32: return f(float());
+        case Element::F16: return f(__half());
+        default: return f(__nv_bfloat16());
+    }
+}
+
+}  // namespace b200fft

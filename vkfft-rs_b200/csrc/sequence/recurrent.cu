@@ -1,0 +1,159 @@
+// The recurrence of linear attention, token by token: the form for single tokens.
+#include <algorithm>
+
+#include "device.cuh"
+
+namespace b200fft {
+
+namespace {
+
+constexpr int kThreads = 128;
+constexpr int kSlice = 32;    // value columns of one CTA
+constexpr int kMaxDim = 256;
+
+// One CTA keeps a [dk, 32] slice of one state in registers: thread (group, lane) holds
+// columns 4 lane .. 4 lane + 3 of rows group, group + 16, ..., so that a state's rows are
+// read and written in 128-byte runs.
+template <typename T, typename O, int ROWS>
+__global__ void __launch_bounds__(kThreads) recurrent_kernel(MixParams p) {
+    __shared__ float sq[kMaxDim], sk[kMaxDim], sv[kSlice];
+    __shared__ float so[kThreads / 32][kSlice];
+    const int slices = (p.dv + kSlice - 1) / kSlice;
+    const int slice = blockIdx.x % slices;
+    const int64_t bh = blockIdx.x / slices;
+    const int h = (int)(bh % p.heads);
+    const int64_t b = bh / p.heads;
+    const int tid = threadIdx.x, lane = tid & 7, group = tid >> 3;
+    const int c0 = slice * kSlice + lane * 4;
+    const Rows rows = rows_of(p.offsets, p.packed_tokens, p.length, b);
+
+    const int64_t slot = p.slots ? p.slots[b] : b;
+    const bool kept = slot >= 0 && slot < p.state_slots;
+    const int64_t state = (slot * p.heads + h) * (int64_t)p.dk * p.dv;
+    const bool wide = p.state_v == 1 && p.dv % 4 == 0 &&
+                      ((reinterpret_cast<uintptr_t>(p.s_in) | reinterpret_cast<uintptr_t>(p.s_out)) & 15) == 0;
+    float s[ROWS][4];
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) {
+        const int row = group + 16 * r;
+        if (p.s_in && kept && row < p.dk && wide && c0 < p.dv) {
+            const float4 v = *reinterpret_cast<const float4 *>(p.s_in + state + (int64_t)row * p.state_k + c0);
+            s[r][0] = v.x, s[r][1] = v.y, s[r][2] = v.z, s[r][3] = v.w;
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                s[r][c] = p.s_in && kept && row < p.dk && c0 + c < p.dv
+                              ? p.s_in[state + (int64_t)row * p.state_k + (c0 + c) * p.state_v]
+                              : 0.f;
+        }
+    }
+    // l in two parts: rounded to one, slow decays would be off by up to 2^-25 a token, always to the same side
+    const float log_decay = p.log_decay[h];
+    const float l = expf(log_decay), l_rest = log_decay > -0.5f ? expm1f(log_decay) - (l - 1.f) : 0.f;
+    const T *q = static_cast<const T *>(p.q.p) + (p.offsets ? 0 : b * p.q.sb) + (h / p.q.per_head) * p.q.sh;
+    const T *k = static_cast<const T *>(p.k.p) + (p.offsets ? 0 : b * p.k.sb) + (h / p.k.per_head) * p.k.sh;
+    const T *v = static_cast<const T *>(p.v.p) + (p.offsets ? 0 : b * p.v.sb) + (h / p.v.per_head) * p.v.sh;
+    O *o = static_cast<O *>(p.o) + (p.offsets ? 0 : b * p.osb) + h * p.osh;
+
+    for (int64_t t = 0; t < rows.count; t++) {
+        const int64_t row = rows.start + (p.reverse ? rows.count - 1 - t : t);
+        for (int i = tid; i < 16 * ROWS; i += kThreads) {
+            sq[i] = i < p.dk ? to_float(q[row * p.q.st + i]) : 0.f;
+            sk[i] = i < p.dk ? p.update * to_float(k[row * p.k.st + i]) : 0.f;
+        }
+        if (tid < kSlice) sv[tid] = slice * kSlice + tid < p.dv ? to_float(v[row * p.v.st + slice * kSlice + tid]) : 0.f;
+        __syncthreads();
+        float acc[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int r = 0; r < ROWS; r++) {
+            const float kk = sk[group + 16 * r], qq = sq[group + 16 * r];
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                if (!p.reverse) s[r][c] = fmaf(s[r][c], l_rest, s[r][c] * l);
+                s[r][c] = fmaf(kk, sv[lane * 4 + c], s[r][c]);
+                acc[c] = fmaf(qq, s[r][c], acc[c]);
+                if (p.reverse) s[r][c] = fmaf(s[r][c], l_rest, s[r][c] * l);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            acc[c] += __shfl_xor_sync(~0u, acc[c], 8);
+            acc[c] += __shfl_xor_sync(~0u, acc[c], 16);
+            if ((tid & 31) < 8) so[tid >> 5][lane * 4 + c] = acc[c];
+        }
+        __syncthreads();
+        if (p.o && tid < kSlice && slice * kSlice + tid < p.dv) {
+            const float sum = so[0][tid] + so[1][tid] + so[2][tid] + so[3][tid];
+            o[row * p.ost + slice * kSlice + tid] = from_float<O>(p.out * sum);
+        }
+    }
+    if (!p.s_out || !kept) return;
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) {
+        const int row = group + 16 * r;
+        if (row >= p.dk) continue;
+        if (wide && c0 < p.dv) {
+            *reinterpret_cast<float4 *>(p.s_out + state + (int64_t)row * p.state_k + c0) =
+                make_float4(s[r][0], s[r][1], s[r][2], s[r][3]);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                if (c0 + c < p.dv) p.s_out[state + (int64_t)row * p.state_k + (c0 + c) * p.state_v] = s[r][c];
+        }
+    }
+}
+
+template <typename T, typename O>
+cudaError_t launch_typed(const MixParams &p, cudaStream_t s) {
+    const unsigned grid = (unsigned)(p.batch * p.heads * ((p.dv + kSlice - 1) / kSlice));
+    before_launch();
+    if (p.dk <= 32)
+        recurrent_kernel<T, O, 2><<<grid, kThreads, 0, s>>>(p);
+    else if (p.dk <= 64)
+        recurrent_kernel<T, O, 4><<<grid, kThreads, 0, s>>>(p);
+    else if (p.dk <= 128)
+        recurrent_kernel<T, O, 8><<<grid, kThreads, 0, s>>>(p);
+    else
+        recurrent_kernel<T, O, 16><<<grid, kThreads, 0, s>>>(p);
+    return cudaGetLastError();
+}
+
+// Sums the partial gradients of the query heads that share a key/value head, in head order.
+template <typename T>
+__global__ void __launch_bounds__(256) share_kernel(ShareParams p) {
+    const int64_t b = blockIdx.y;
+    const Rows rows = rows_of(p.offsets, p.packed_tokens, p.length, b);
+    const int64_t per = (int64_t)p.kv_heads * p.dim, n = rows.count * per;
+    const int64_t first = rows.start + (p.offsets ? 0 : b * p.length);
+    T *dst = static_cast<T *>(p.dst) + (p.offsets ? 0 : b * p.sb);
+    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t t = i / per;
+        const int r = (int)(i - t * per), g = r / p.dim, d = r - g * p.dim;
+        const float *src = p.src + ((first + t) * p.kv_heads + g) * p.share * (int64_t)p.dim + d;
+        float s = 0;
+        for (int j = 0; j < p.share; j++) s += src[j * p.dim];
+        dst[(rows.start + t) * p.st + g * p.sh + d] = from_float<T>(s);
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_recurrent(const MixParams &p, Element e, bool out_f32, cudaStream_t s) {
+    return with_element(e, [&](auto t) {
+        using T = decltype(t);
+        return out_f32 ? launch_typed<T, float>(p, s) : launch_typed<T, T>(p, s);
+    });
+}
+
+cudaError_t launch_share(const ShareParams &p, Element e, cudaStream_t s) {
+    return with_element(e, [&](auto t) {
+        using T = decltype(t);
+        const int64_t n = p.length * p.kv_heads * p.dim;
+        const dim3 grid((unsigned)std::min<int64_t>((n + 255) / 256, 4096), (unsigned)p.batch);
+        before_launch();
+        share_kernel<T><<<grid, 256, 0, s>>>(p);
+        return cudaGetLastError();
+    });
+}
+
+}  // namespace b200fft

@@ -1,0 +1,305 @@
+// Configurations, checks and execution of the sequence operators.
+#include "sequence.hpp"
+
+#include <algorithm>
+#include <cmath>
+
+namespace b200fft {
+
+static void check(cudaError_t e, const char *what) {
+    if (e != cudaSuccess) fail_runtime(std::string(what) + " failed: " + cudaGetErrorString(e));
+}
+
+static Element element_from_c(int32_t v, const char *what) {
+    if (v < 0 || v > 2) fail_value_range(what);
+    return static_cast<Element>(v);
+}
+
+static void aligned(const void *p, size_t to, const char *what) {
+    if (reinterpret_cast<uintptr_t>(p) % to)
+        throw FftError(B200FFT_VALUE_OUT_OF_RANGE, std::string(what) + " must be aligned to its elements");
+}
+
+// A pointer that has to be there (unless it is optional) and to be aligned to `to` bytes.
+static void tensor(const void *p, size_t to, const char *what, bool required = true) {
+    if (!p && required) throw FftError(B200FFT_VALUE_OUT_OF_RANGE, std::string(what) + " must not be null");
+    aligned(p, to, what);
+}
+
+constexpr uint64_t kMostElements = uint64_t(1) << 46;  // element offsets, doubled or times 8 bytes, stay in 64 bits
+
+static int64_t bounded(uint64_t v, uint64_t most, const char *what) {
+    if (v > most) fail_value_range(what);
+    return static_cast<int64_t>(v);
+}
+
+// ---- layer normalisation --------------------------------------------------------------
+
+LayerNorm LayerNorm::from_c(const b200fft_layer_norm_config &c) {
+    LayerNorm n{};
+    if (c.features == 0) throw FftError(B200FFT_ZERO_LENGTH, "layer normalisation needs at least one feature");
+    if (c.rows == 0) throw FftError(B200FFT_ZERO_BATCH_COUNT, "layer normalisation needs at least one row");
+    n.features = bounded(c.features, uint64_t(1) << 30, "features");
+    n.rows = bounded(c.rows, uint64_t(1) << 40, "rows");
+    n.x_stride = c.input_row_stride ? bounded(c.input_row_stride, kMostElements, "input row stride") : n.features;
+    n.y_stride = c.output_row_stride ? bounded(c.output_row_stride, kMostElements, "output row stride") : n.features;
+    if (n.x_stride < n.features) fail_value_range("input row stride");
+    if (n.y_stride < n.features) fail_value_range("output row stride");
+    if (checked_mul(c.rows, (size_t)std::max(n.x_stride, n.y_stride), "layer normalisation extent") > kMostElements)
+        fail_value_range("layer normalisation extent");
+    if (!(c.epsilon >= 0.f) || !std::isfinite(c.epsilon)) fail_value_range("epsilon");
+    n.epsilon = c.epsilon;
+    n.element = element_from_c(c.element_type, "element type");
+    n.parameter = element_from_c(c.parameter_type, "parameter type");
+    return n;
+}
+
+int LayerNorm::partials() const { return (int)std::clamp<int64_t>(rows / 64, 1, 64); }
+
+size_t LayerNorm::backward_workspace() const { return (size_t)partials() * features * 2 * sizeof(float); }
+
+void execute_layer_norm(Context *ctx, const LayerNorm &n, const NormParams &args, cudaStream_t stream) {
+    const size_t e = element_bytes(n.element), pe = element_bytes(n.parameter);
+    tensor(args.x, e, "input");
+    tensor(args.y, e, "output");
+    tensor(args.w, pe, "weight", false);
+    tensor(args.b, pe, "bias", false);
+    tensor(args.mean, 4, "mean", false);
+    tensor(args.rstd, 4, "rstd", false);
+    NormParams p = args;
+    p.rows = n.rows;
+    p.features = n.features;
+    p.xs = n.x_stride;
+    p.ys = n.y_stride;
+    p.epsilon = n.epsilon;
+    check(cudaSetDevice(ctx->device), "cudaSetDevice");
+    std::lock_guard<std::mutex> l(ctx->mu);
+    check(launch_norm(p, n.element, n.parameter, stream ? stream : ctx->stream), "kernel launch");
+}
+
+void execute_layer_norm_grad(Context *ctx, const LayerNorm &n, NormGradParams p, void *workspace, cudaStream_t stream) {
+    const size_t e = element_bytes(n.element), pe = element_bytes(n.parameter);
+    tensor(p.x, e, "input");
+    tensor(p.dy, e, "output gradient");
+    tensor(p.mean, 4, "mean");
+    tensor(p.rstd, 4, "rstd");
+    tensor(p.w, pe, "weight", false);
+    tensor(p.dx, e, "input gradient", false);
+    tensor(p.dw, pe, "weight gradient", false);
+    tensor(p.db, pe, "bias gradient", false);
+    tensor(workspace, 16, "workspace", false);
+    p.rows = n.rows;
+    p.features = n.features;
+    p.xs = n.x_stride;
+    p.ys = n.y_stride;
+    p.partials = n.partials();
+    check(cudaSetDevice(ctx->device), "cudaSetDevice");
+    std::lock_guard<std::mutex> l(ctx->mu);
+    if (!workspace && (p.dw || p.db)) workspace = context_scratch(ctx, n.backward_workspace());
+    p.part_w = static_cast<float *>(workspace);
+    p.part_b = p.part_w + (size_t)p.partials * n.features;
+    check(launch_norm_grad(p, n.element, n.parameter, stream ? stream : ctx->stream), "kernel launch");
+}
+
+// ---- linear attention -----------------------------------------------------------------
+
+constexpr uint64_t kMostDim = 256;
+
+static AttentionTensor layout(const uint64_t (&strides)[3], bool packed, int64_t length, int64_t heads, int64_t dim,
+                              int64_t batch, int64_t packed_tokens, const char *what) {
+    AttentionTensor t{};
+    t.dim = dim;
+    t.sh = strides[2] ? bounded(strides[2], kMostElements, what) : dim;
+    t.st = strides[1] ? bounded(strides[1], kMostElements, what) : heads * dim;
+    if (t.sh < dim || t.st < dim) fail_value_range(what);
+    const size_t rows = checked_mul((size_t)(packed ? packed_tokens : length), (size_t)t.st, what);
+    t.sb = strides[0] ? bounded(strides[0], kMostElements, what) : bounded(rows, kMostElements, what);
+    const size_t all = checked_add(checked_add(packed ? 0 : checked_mul((size_t)(batch - 1), (size_t)t.sb, what), rows, what),
+                                   checked_mul((size_t)heads, (size_t)t.sh, what), what);
+    if (all > kMostElements) fail_value_range(what);
+    return t;
+}
+
+LinearAttention LinearAttention::from_c(const b200fft_linear_attention_config &c) {
+    LinearAttention a{};
+    if (c.batch_count == 0) throw FftError(B200FFT_ZERO_BATCH_COUNT, "linear attention needs at least one sequence");
+    if (c.length == 0 || c.heads == 0 || c.key_value_heads == 0 || c.key_dim == 0 || c.value_dim == 0)
+        throw FftError(B200FFT_ZERO_LENGTH, "linear attention needs a length, heads and head dimensions of at least one");
+    a.batch = bounded(c.batch_count, 65535, "batch count");
+    a.length = bounded(c.length, (uint64_t(1) << 31) - 1, "length");
+    a.heads = bounded(c.heads, 65535, "heads");
+    a.kv_heads = bounded(c.key_value_heads, c.heads, "key/value heads");
+    if (a.heads % a.kv_heads) fail_value_range("key/value heads");
+    if (c.key_dim > kMostDim || c.value_dim > kMostDim)
+        fail_unsupported("linear attention supports key and value dimensions of at most 256");
+    a.key_dim = (int64_t)c.key_dim;
+    a.value_dim = (int64_t)c.value_dim;
+    a.packed = c.packed != 0;
+    a.packed_tokens = a.packed ? bounded(c.packed_tokens, (uint64_t(1) << 40), "packed tokens") : 0;
+    a.slots = c.state_slots ? bounded(c.state_slots, (uint64_t(1) << 31) - 1, "state slots") : a.batch;
+    // one launch holds at most 2^31 - 1 CTAs: eight slices of 32 value columns for each head of each sequence
+    if (a.batch * a.heads > (int64_t(1) << 28) - 1) fail_value_range("batch count times heads");
+    if ((uint64_t)(std::max(a.slots, a.batch) * a.heads) > kMostElements / (kMostDim * kMostDim)) fail_value_range("state slots");
+    if (!std::isfinite(c.scale)) fail_value_range("scale");
+    a.scale = c.scale;
+    a.element = element_from_c(c.element_type, "element type");
+    a.q = layout(c.query_strides, a.packed, a.length, a.heads, a.key_dim, a.batch, a.packed_tokens, "query strides");
+    a.k = layout(c.key_strides, a.packed, a.length, a.kv_heads, a.key_dim, a.batch, a.packed_tokens, "key strides");
+    a.v = layout(c.value_strides, a.packed, a.length, a.kv_heads, a.value_dim, a.batch, a.packed_tokens, "value strides");
+    a.o = layout(c.output_strides, a.packed, a.length, a.heads, a.value_dim, a.batch, a.packed_tokens, "output strides");
+    if ((uint64_t)a.tokens() > kMostElements / (uint64_t)(a.heads * kMostDim)) fail_value_range("tokens");
+    return a;
+}
+
+size_t LinearAttention::workspace() const { return 0; }
+
+size_t LinearAttention::backward_workspace() const {
+    // f32 partial gradients of every query head, where key/value heads are shared
+    return share() > 1 ? (size_t)tokens() * heads * (key_dim + value_dim) * sizeof(float) : 0;
+}
+
+static MixOperand operand(const void *p, const AttentionTensor &t, int per_head) { return {p, t.sb, t.st, t.sh, per_head}; }
+
+static MixParams common(const Context *ctx, const LinearAttention &a, const float *log_decay, const int64_t *offsets) {
+    MixParams p{};
+    p.log_decay = log_decay;
+    p.offsets = offsets;
+    p.length = a.length;
+    p.packed_tokens = a.packed_tokens;
+    p.batch = a.batch;
+    p.heads = (int)a.heads;
+    p.err = ctx->d_err;
+    return p;
+}
+
+static void output_to(MixParams &p, void *o, const AttentionTensor &t) {
+    p.o = o;
+    p.osb = t.sb;
+    p.ost = t.st;
+    p.osh = t.sh;
+}
+
+void execute_linear_attention(Context *ctx, const LinearAttention &a, const b200fft_linear_attention_buffers &b,
+                              void *workspace, cudaStream_t stream) {
+    const size_t e = element_bytes(a.element);
+    const bool some = a.tokens() > 0;
+    tensor(b.query, e, "query", some);
+    tensor(b.key, e, "key", some);
+    tensor(b.value, e, "value", some);
+    tensor(b.output, e, "output", some);
+    tensor(b.log_decay, 4, "log_decay");
+    tensor(b.sequence_offsets, 8, "sequence_offsets", a.packed);
+    tensor(b.state_slots, 4, "state_slots", false);
+    tensor(b.initial_state, 4, "initial_state", false);
+    tensor(b.final_state, 4, "final_state", false);
+    tensor(workspace, 16, "workspace", false);
+    check(cudaSetDevice(ctx->device), "cudaSetDevice");
+    std::lock_guard<std::mutex> l(ctx->mu);
+    if (!stream) stream = ctx->stream;
+    MixParams p = common(ctx, a, b.log_decay, a.packed ? b.sequence_offsets : nullptr);
+    p.q = operand(b.query, a.q, 1);
+    p.k = operand(b.key, a.k, a.share());
+    p.v = operand(b.value, a.v, a.share());
+    output_to(p, b.output, a.o);
+    p.slots = b.state_slots;
+    p.state_slots = a.slots;
+    p.s_in = b.initial_state;
+    p.s_out = b.final_state;
+    p.state_k = a.value_dim;
+    p.state_v = 1;
+    p.dk = (int)a.key_dim;
+    p.dv = (int)a.value_dim;
+    p.update = 1.f;
+    p.out = a.scale;
+    check(launch_recurrent(p, a.element, false, stream), "kernel launch");
+}
+
+void execute_linear_attention_grad(Context *ctx, const LinearAttention &a,
+                                   const b200fft_linear_attention_gradients &g, void *workspace, cudaStream_t stream) {
+    const size_t e = element_bytes(a.element);
+    const bool some = a.tokens() > 0;
+    tensor(g.query, e, "query", some);
+    tensor(g.key, e, "key", some);
+    tensor(g.value, e, "value", some);
+    tensor(g.output_gradient, e, "output_gradient", some);
+    tensor(g.log_decay, 4, "log_decay");
+    tensor(g.sequence_offsets, 8, "sequence_offsets", a.packed);
+    tensor(g.initial_state, 4, "initial_state", false);
+    tensor(g.final_state_gradient, 4, "final_state_gradient", false);
+    tensor(g.query_gradient, e, "query_gradient", false);
+    tensor(g.key_gradient, e, "key_gradient", false);
+    tensor(g.value_gradient, e, "value_gradient", false);
+    tensor(g.initial_state_gradient, 4, "initial_state_gradient", false);
+    tensor(workspace, 16, "workspace", false);
+    check(cudaSetDevice(ctx->device), "cudaSetDevice");
+    std::lock_guard<std::mutex> l(ctx->mu);
+    if (!stream) stream = ctx->stream;
+    const int share = a.share();
+    if (!workspace && a.backward_workspace()) workspace = context_scratch(ctx, a.backward_workspace());
+    const MixParams base = common(ctx, a, g.log_decay, a.packed ? g.sequence_offsets : nullptr);
+    const MixOperand q = operand(g.query, a.q, 1), k = operand(g.key, a.k, share), v = operand(g.value, a.v, share),
+                     d = operand(g.output_gradient, a.o, 1);
+
+    if (g.query_gradient) {  // dq = scale * the operator on (do, v, k), from the transposed initial state
+        MixParams p = base;
+        p.q = d, p.k = v, p.v = k;
+        output_to(p, g.query_gradient, a.q);
+        p.s_in = g.initial_state;
+        p.state_slots = a.batch;
+        p.state_k = 1;
+        p.state_v = a.value_dim;
+        p.dk = (int)a.value_dim;
+        p.dv = (int)a.key_dim;
+        p.update = 1.f;
+        p.out = a.scale;
+        check(launch_recurrent(p, a.element, false, stream), "kernel launch");
+    }
+    // dk and dv run from the last token back; their state is the state's gradient
+    auto late = [&](const MixOperand &rq, const MixOperand &rk, const MixOperand &rv, int64_t dk, int64_t dv,
+                    int64_t state_k, int64_t state_v, void *out, const AttentionTensor &t, float *partial, float *s_out) {
+        MixParams p = base;
+        p.reverse = 1;
+        p.q = rq, p.k = rk, p.v = rv;
+        p.s_in = g.final_state_gradient;
+        p.s_out = s_out;
+        p.state_slots = a.batch;
+        p.state_k = state_k;
+        p.state_v = state_v;
+        p.dk = (int)dk;
+        p.dv = (int)dv;
+        p.update = a.scale;
+        p.out = 1.f;
+        if (share == 1 || !out) {
+            output_to(p, out, t);
+        } else {
+            const AttentionTensor dense{a.length * a.heads * dv, a.heads * dv, dv, dv};
+            output_to(p, partial, dense);
+        }
+        check(launch_recurrent(p, a.element, share > 1, stream), "kernel launch");
+        if (share > 1 && out) {
+            ShareParams sp{};
+            sp.src = partial;
+            sp.dst = out;
+            sp.sb = t.sb, sp.st = t.st, sp.sh = t.sh;
+            sp.offsets = base.offsets;
+            sp.length = a.length;
+            sp.packed_tokens = a.packed_tokens;
+            sp.batch = a.batch;
+            sp.kv_heads = (int)a.kv_heads;
+            sp.share = share;
+            sp.dim = (int)dv;
+            check(launch_share(sp, a.element, stream), "kernel launch");
+        }
+    };
+    float *part_k = static_cast<float *>(workspace), *part_v = part_k + (share > 1 ? a.tokens() * a.heads * a.key_dim : 0);
+    // the state's own gradient comes out of the last pass that reads the final state's, which it may replace
+    if (g.key_gradient)
+        late(v, d, q, a.value_dim, a.key_dim, 1, a.value_dim, g.key_gradient, a.k, part_k,
+             g.value_gradient ? nullptr : g.initial_state_gradient);
+    if (g.value_gradient || (g.initial_state_gradient && !g.key_gradient)) {
+        void *out = g.value_gradient;
+        late(k, q, d, a.key_dim, a.value_dim, a.value_dim, 1, out, a.v, part_v, g.initial_state_gradient);
+    }
+}
+
+}  // namespace b200fft

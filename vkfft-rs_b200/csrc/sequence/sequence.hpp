@@ -1,0 +1,126 @@
+// Sequence operators: layer normalisation and linear attention with a decay per head.
+// Host-side configurations, the kernels' parameters and their launch functions.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+#include "../runtime.hpp"
+
+namespace b200fft {
+
+// Streaming multiprocessors of the target (B200): plans, workspaces included, are made
+// without a device, so grids are sized for it.
+constexpr int kSms = 148;
+
+enum class Element : int { F32 = 0, F16 = 1, BF16 = 2 };
+inline size_t element_bytes(Element e) { return e == Element::F32 ? 4 : 2; }
+
+// ---- layer normalisation ----------------------------------------------------------
+
+struct LayerNorm {
+    int64_t rows, features, x_stride, y_stride;
+    float epsilon;
+    Element element, parameter;
+    static LayerNorm from_c(const b200fft_layer_norm_config &c);
+    int partials() const;  // row strips whose sums the backward pass keeps apart
+    size_t backward_workspace() const;
+};
+
+struct NormParams {
+    const void *x, *w, *b;
+    void *y;
+    float *mean, *rstd;
+    int64_t rows, xs, ys;
+    int64_t features;
+    float epsilon;
+};
+
+struct NormGradParams {
+    const void *x, *w, *dy;
+    const float *mean, *rstd;
+    void *dx, *dw, *db;
+    float *part_w, *part_b;  // [partials][features]
+    int64_t rows, xs, ys;
+    int64_t features;
+    int partials;
+};
+
+cudaError_t launch_norm(const NormParams &p, Element e, Element param, cudaStream_t s);
+cudaError_t launch_norm_grad(const NormGradParams &p, Element e, Element param, cudaStream_t s);
+
+// ---- linear attention -----------------------------------------------------------------
+
+struct AttentionTensor {
+    int64_t sb, st, sh;  // elements between batches, tokens, heads
+    int64_t dim;
+};
+
+struct LinearAttention {
+    int64_t batch, length, heads, kv_heads, key_dim, value_dim, packed_tokens, slots;
+    bool packed;
+    Element element;
+    float scale;
+    AttentionTensor q, k, v, o;
+    static LinearAttention from_c(const b200fft_linear_attention_config &c);
+    int64_t tokens() const { return packed ? packed_tokens : batch * length; }
+    int share() const { return static_cast<int>(heads / kv_heads); }
+    size_t workspace() const;
+    size_t backward_workspace() const;
+};
+
+// One operand of the recurrence: query head h reads head h / per_head of the tensor.
+struct MixOperand {
+    const void *p;
+    int64_t sb, st, sh;
+    int per_head;
+};
+
+// The recurrence all passes share, over the rows of each sequence in processing order
+// (reverse: from the last token to the first):
+//   early (forward, dq):     S <- l S + update (k x v);  o = out (q . S)
+//   late  (reverse: dk, dv): S <- S + update (k x v);    o = out (q . S);  S <- l S
+// q, k, v, o are the roles of this pass: the gradients run it with others in their place.
+struct MixParams {
+    MixOperand q, k, v;
+    void *o;
+    int64_t osb, ost, osh;
+    const float *log_decay;
+    const int64_t *offsets;
+    const int32_t *slots;
+    const float *s_in;
+    float *s_out;
+    int64_t state_k, state_v;  // strides of a state in its role's key and value dimension
+    int64_t state_slots;
+    int64_t length, packed_tokens;
+    int64_t batch;
+    int heads, dk, dv;
+    int reverse;  // from the last token, decay after the output
+    float update, out;
+    int *err;
+};
+
+// out_f32: o holds f32 whatever the element type (partial gradients of shared heads)
+cudaError_t launch_recurrent(const MixParams &p, Element e, bool out_f32, cudaStream_t s);
+
+// dst[.., g, d] = sum over the share query heads of src[token, g * share + j, d]
+struct ShareParams {
+    const float *src;  // [tokens][kv_heads * share][dim], token as in the workspace
+    void *dst;
+    int64_t sb, st, sh;
+    const int64_t *offsets;
+    int64_t length, packed_tokens, batch;
+    int kv_heads, share, dim;
+};
+cudaError_t launch_share(const ShareParams &p, Element e, cudaStream_t s);
+
+void execute_layer_norm(Context *ctx, const LayerNorm &n, const NormParams &p, cudaStream_t stream);
+void execute_layer_norm_grad(Context *ctx, const LayerNorm &n, NormGradParams p, void *workspace, cudaStream_t stream);
+void execute_linear_attention(Context *ctx, const LinearAttention &a, const b200fft_linear_attention_buffers &b,
+                              void *workspace, cudaStream_t stream);
+void execute_linear_attention_grad(Context *ctx, const LinearAttention &a,
+                                   const b200fft_linear_attention_gradients &g, void *workspace, cudaStream_t stream);
+
+}  // namespace b200fft

@@ -16,8 +16,11 @@ path, and importing this module on a machine without the built library fails.
 import ctypes
 import enum
 import os
+import sys
 
 import numpy as np
+
+from . import sequence as _sequence
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _PKG = os.path.dirname(_HERE)
@@ -287,6 +290,7 @@ def library():
         "b200fft_ticket_wait": ([vp], i32),
         "b200fft_ticket_destroy": ([vp], None),
     }
+    sigs.update(_sequence.signatures())
     for name, (args, res) in sigs.items():
         fn = getattr(lib, name)
         fn.argtypes = args
@@ -962,7 +966,7 @@ class AsyncTransformTicket:
             self._h = None
 
 
-class CudaExecutionContext:
+class CudaExecutionContext(_sequence.SequenceExecution):
     """backend/cuda/runtime.rs:959-2840"""
 
     def __init__(self, device_index=0):
@@ -1078,6 +1082,13 @@ class CudaExecutionContext:
 
 
 STATIC_WORKSPACE_BYTES = 16 << 20
+
+_sequence._package.append(sys.modules[__name__])
+ElementType = _sequence.ElementType
+LayerNormConfig = _sequence.LayerNormConfig
+LayerNormIr = _sequence.LayerNormIr
+LinearAttentionConfig = _sequence.LinearAttentionConfig
+LinearAttentionIr = _sequence.LinearAttentionIr
 
 
 def exported_symbols():

@@ -1,0 +1,243 @@
+"""Sequence operators of the C ABI: layer normalisation and linear attention with a decay per head.
+
+They stand beside the FFT convolution in a sequence-mixing block: the convolution's filter
+is fixed, the attention's depends on the data.  As for transforms, a configuration is built
+by `with_*` methods, an `...Ir` is made of it once, and a context executes that on device
+pointers, ordered on a stream:
+
+    cfg = LinearAttentionConfig(length, heads, key_dim, value_dim).with_element_type(ElementType.BF16)
+    ir = LinearAttentionIr.build(cfg, ctx.device_profile())
+    ctx.execute_linear_attention(ir, q, k, v, log_decay, o, final_state_ptr=s, stream=stream)
+
+stream=0 is the context's own stream, as for transforms; stream=1 is CUDA's legacy default
+stream.  A pointer of 0 leaves an optional tensor out.
+"""
+import ctypes
+import enum
+
+u64 = ctypes.c_uint64
+i32 = ctypes.c_int32
+vp = ctypes.c_void_p
+
+
+class ElementType(enum.IntEnum):
+    F32 = 0
+    F16 = 1
+    BF16 = 2
+
+
+class _LayerNorm(ctypes.Structure):
+    _fields_ = [("rows", u64), ("features", u64), ("input_row_stride", u64), ("output_row_stride", u64),
+                ("epsilon", ctypes.c_float), ("element_type", i32), ("parameter_type", i32), ("_reserved", i32)]
+
+
+class _LinearAttention(ctypes.Structure):
+    _fields_ = [("batch_count", u64), ("length", u64), ("heads", u64), ("key_value_heads", u64), ("key_dim", u64),
+                ("value_dim", u64), ("packed", i32), ("element_type", i32), ("packed_tokens", u64),
+                ("state_slots", u64), ("scale", ctypes.c_float), ("_reserved", i32),
+                ("query_strides", u64 * 3), ("key_strides", u64 * 3), ("value_strides", u64 * 3),
+                ("output_strides", u64 * 3)]
+
+
+class _Buffers(ctypes.Structure):
+    _fields_ = [(n, vp) for n in ("query", "key", "value", "log_decay", "sequence_offsets", "state_slots",
+                                  "initial_state", "output", "final_state")]
+
+
+class _Gradients(ctypes.Structure):
+    _fields_ = [(n, vp) for n in ("query", "key", "value", "log_decay", "sequence_offsets", "initial_state",
+                                  "output_gradient", "final_state_gradient", "query_gradient", "key_gradient",
+                                  "value_gradient", "initial_state_gradient")]
+
+
+def signatures():
+    P = ctypes.POINTER
+    return {
+        "b200fft_layer_norm_config_init": ([P(_LayerNorm), u64, u64], i32),
+        "b200fft_layer_norm_config_validate": ([P(_LayerNorm)], i32),
+        "b200fft_layer_norm_build": ([P(_LayerNorm), vp, P(vp)], i32),
+        "b200fft_layer_norm_destroy": ([vp], None),
+        "b200fft_layer_norm_backward_workspace_bytes": ([vp], u64),
+        "b200fft_execute_layer_norm": ([vp] * 9, i32),
+        "b200fft_execute_layer_norm_backward": ([vp] * 12, i32),
+        "b200fft_linear_attention_config_init": ([P(_LinearAttention), u64, u64, u64, u64], i32),
+        "b200fft_linear_attention_config_validate": ([P(_LinearAttention)], i32),
+        "b200fft_linear_attention_build": ([P(_LinearAttention), vp, P(vp)], i32),
+        "b200fft_linear_attention_destroy": ([vp], None),
+        "b200fft_linear_attention_workspace_bytes": ([vp], u64),
+        "b200fft_linear_attention_backward_workspace_bytes": ([vp], u64),
+        "b200fft_execute_linear_attention": ([vp, vp, P(_Buffers), vp, vp], i32),
+        "b200fft_execute_linear_attention_backward": ([vp, vp, P(_Gradients), vp, vp], i32),
+    }
+
+
+_package = []  # the vkfft_rs module, set when it has been imported
+
+
+def _api():
+    return _package[0]
+
+
+class _Config:
+    def _copy(self):
+        c = type(self).__new__(type(self))
+        c._s = type(self._s)()
+        ctypes.memmove(ctypes.byref(c._s), ctypes.byref(self._s), ctypes.sizeof(self._s))
+        return c
+
+    def _set(self, **kw):
+        c = self._copy()
+        for k, v in kw.items():
+            setattr(c._s, k, v)
+        return c
+
+    def with_element_type(self, element_type):
+        return self._set(element_type=int(element_type))
+
+
+class LayerNormConfig(_Config):
+    """Layer normalisation over the last axis of [rows, features]."""
+
+    def __init__(self, rows, features):
+        self._s = _LayerNorm()
+        api = _api()
+        api._check(api.library().b200fft_layer_norm_config_init(ctypes.byref(self._s), int(rows), int(features)))
+
+    def with_parameter_type(self, parameter_type):
+        return self._set(parameter_type=int(parameter_type))
+
+    def with_epsilon(self, epsilon):
+        return self._set(epsilon=float(epsilon))
+
+    def with_input_row_stride(self, stride):
+        return self._set(input_row_stride=int(stride))
+
+    def with_output_row_stride(self, stride):
+        return self._set(output_row_stride=int(stride))
+
+    def validate(self):
+        api = _api()
+        api._check(api.library().b200fft_layer_norm_config_validate(ctypes.byref(self._s)))
+
+
+class LinearAttentionConfig(_Config):
+    """S_t = exp(log_decay) S_(t-1) + k_t v_t^T, o_t = scale S_t^T q_t; scale starts as key_dim ** -0.5."""
+
+    def __init__(self, length, heads, key_dim, value_dim):
+        self._s = _LinearAttention()
+        api = _api()
+        api._check(api.library().b200fft_linear_attention_config_init(
+            ctypes.byref(self._s), int(length), int(heads), int(key_dim), int(value_dim)))
+
+    def with_batch_count(self, n):
+        return self._set(batch_count=int(n))
+
+    def with_key_value_heads(self, n):
+        return self._set(key_value_heads=int(n))
+
+    def with_scale(self, scale):
+        return self._set(scale=float(scale))
+
+    def with_packed_tokens(self, tokens):
+        """Sequences of up to `length` tokens stand behind one another in `tokens` rows."""
+        return self._set(packed=1, packed_tokens=int(tokens))
+
+    def with_state_slots(self, n):
+        """The state buffers hold n states; each sequence names its slot."""
+        return self._set(state_slots=int(n))
+
+    def _strides(self, name, batch, token, head):
+        c = self._copy()
+        getattr(c._s, name)[:] = [int(batch), int(token), int(head)]
+        return c
+
+    def with_query_strides(self, batch, token, head):
+        return self._strides("query_strides", batch, token, head)
+
+    def with_key_strides(self, batch, token, head):
+        return self._strides("key_strides", batch, token, head)
+
+    def with_value_strides(self, batch, token, head):
+        return self._strides("value_strides", batch, token, head)
+
+    def with_output_strides(self, batch, token, head):
+        return self._strides("output_strides", batch, token, head)
+
+    def validate(self):
+        api = _api()
+        api._check(api.library().b200fft_linear_attention_config_validate(ctypes.byref(self._s)))
+
+
+class _Ir:
+    def __init__(self, handle, config):
+        self._h = handle
+        self._destroy = getattr(_api().library(), f"b200fft_{self._name}_destroy")
+        self.config = config
+
+    @classmethod
+    def build(cls, config, device):
+        api = _api()
+        h = vp()
+        api._check(getattr(api.library(), f"b200fft_{cls._name}_build")(
+            ctypes.byref(config._s), ctypes.byref(device._c()), ctypes.byref(h)))
+        return cls(h, config)
+
+    def __del__(self):
+        h, self._h = getattr(self, "_h", None), None
+        if h:
+            self._destroy(h)
+
+    @property
+    def backward_workspace_bytes(self):
+        return int(getattr(_api().library(), f"b200fft_{self._name}_backward_workspace_bytes")(self._h))
+
+
+class LayerNormIr(_Ir):
+    _name = "layer_norm"
+    workspace_bytes = 0  # of the forward pass
+
+
+class LinearAttentionIr(_Ir):
+    _name = "linear_attention"
+
+    @property
+    def workspace_bytes(self):
+        return int(_api().library().b200fft_linear_attention_workspace_bytes(self._h))
+
+
+class SequenceExecution:
+    """The sequence operators of a CudaExecutionContext."""
+
+    def execute_layer_norm(self, ir, input_ptr, output_ptr, weight_ptr=0, bias_ptr=0, mean_ptr=0, rstd_ptr=0, stream=0):
+        """y = (x - mean) rstd weight + bias; mean and rstd (f32) are written where given."""
+        api = _api()
+        api._check(api._lib.b200fft_execute_layer_norm(self._h, ir._h, input_ptr, weight_ptr, bias_ptr, output_ptr,
+                                                       mean_ptr, rstd_ptr, stream))
+
+    def execute_layer_norm_backward(self, ir, input_ptr, mean_ptr, rstd_ptr, output_gradient_ptr, weight_ptr=0,
+                                    input_gradient_ptr=0, weight_gradient_ptr=0, bias_gradient_ptr=0,
+                                    workspace_ptr=0, stream=0):
+        api = _api()
+        api._check(api._lib.b200fft_execute_layer_norm_backward(
+            self._h, ir._h, input_ptr, weight_ptr, mean_ptr, rstd_ptr, output_gradient_ptr, input_gradient_ptr,
+            weight_gradient_ptr, bias_gradient_ptr, workspace_ptr, stream))
+
+    def execute_linear_attention(self, ir, query_ptr, key_ptr, value_ptr, log_decay_ptr, output_ptr,
+                                 initial_state_ptr=0, final_state_ptr=0, sequence_offsets_ptr=0, state_slots_ptr=0,
+                                 workspace_ptr=0, stream=0):
+        """Whole sequences, or (length 1) one new token of each, from initial_state to final_state."""
+        api = _api()
+        b = _Buffers(query_ptr, key_ptr, value_ptr, log_decay_ptr, sequence_offsets_ptr, state_slots_ptr,
+                     initial_state_ptr, output_ptr, final_state_ptr)
+        api._check(api._lib.b200fft_execute_linear_attention(self._h, ir._h, b, workspace_ptr, stream))
+
+    def execute_linear_attention_backward(self, ir, query_ptr, key_ptr, value_ptr, log_decay_ptr, output_gradient_ptr,
+                                          query_gradient_ptr=0, key_gradient_ptr=0, value_gradient_ptr=0,
+                                          initial_state_ptr=0, final_state_gradient_ptr=0,
+                                          initial_state_gradient_ptr=0, sequence_offsets_ptr=0, workspace_ptr=0,
+                                          stream=0):
+        api = _api()
+        g = _Gradients(query_ptr, key_ptr, value_ptr, log_decay_ptr, sequence_offsets_ptr, initial_state_ptr,
+                       output_gradient_ptr, final_state_gradient_ptr, query_gradient_ptr, key_gradient_ptr,
+                       value_gradient_ptr, initial_state_gradient_ptr)
+        api._check(api._lib.b200fft_execute_linear_attention_backward(self._h, ir._h, g, workspace_ptr, stream))
