@@ -1,0 +1,1041 @@
+// Linear attention by chunks of 128 tokens on the tensor cores (bf16).
+//
+// With the state S that enters a chunk (rows i, j of the chunk, l the head's decay)
+//   o_i = out * ( sum_{j <= i} l^(i-j) (q_i . k_j) v_j  +  l^(i+1) S^T q_i )
+//   S  <- l^128 S + sum_j l^(127-j) k_j v_j^T
+// and, from the last token back (the gradients dk and dv), the mirror image of it.
+//
+// A CTA takes one segment (some chunks) of one head of one sequence and keeps S in
+// registers, in f32.  Per chunk, with the matrices that the tensor cores see in brackets:
+//   scores  [Q K^T]            128 x 128, decayed, rounded to bf16 in tensor memory (P)
+//   inside  [P V]              128 x dv
+//   before  [Q S]              128 x dv, S rounded to bf16 in shared memory; rows decayed in f32
+//   update  [W^T V]            dk x dv, W_j = l^(127-j) k_j as four bf16 terms that hold the 24
+//                              bits of the f32 product: the state is an f32 result and stays one
+// The two roundings (P, S) and the result's own are each half a unit of bf16: the result is
+// within sqrt(3) of the rounding that any bf16 result has.
+#include <algorithm>
+
+#include "tcgen05.cuh"
+
+namespace b200fft {
+
+namespace {
+
+constexpr int kChunk = 128;
+// 16 warps of arithmetic; a warpgroup in which one thread issues the products, one moves the tiles and two
+// warps look the values over.  (With one thread of the former issuing, its warp held all others up: 5000 of
+// 11700 clocks a chunk.)  640 x 96 registers at launch; afterwards 512 x 104 + 128 x 64.
+constexpr int kComputeWarps = 16, kThreads = (kComputeWarps + 4) * 32;
+constexpr int kComputeRegisters = 104, kOtherRegisters = 64;
+static_assert(kComputeWarps * 32 * kComputeRegisters + 128 * kOtherRegisters <= kThreads * 96, "register shares");
+constexpr int kGroups = kComputeWarps / 4;  // each has all 128 tensor memory lanes and a share of the columns
+constexpr uint32_t kTmemColumns = 512;
+// tensor memory columns: scores and P; results; state update; W terms
+constexpr uint32_t kX = 0, kY = 128, kZ = 256, kW = 384;
+constexpr int kPanel = kChunk * 128;  // bytes of 128 rows x 64 elements
+
+struct ChunkParams {
+    MixParams p;
+    float *segments;  // [batch][heads][count][dk][dv]: first each segment's own sum, then the state that enters it
+    int count;        // segments of a sequence
+    int chunks;       // chunks of a segment
+    int out_f32;
+};
+
+struct Maps {
+    CUtensorMap q, k, v, o;
+};
+
+constexpr int kMostShared = 227 * 1024 - 2048;  // of a CTA, beside its static arrays
+
+template <int DK, int DV>
+struct Layout {
+    static constexpr int q = 0;
+    static constexpr int k = (DK / 64) * kPanel;
+    static constexpr int v = k + (DK / 64) * kPanel;
+    static constexpr int stage = v + (DV / 64) * kPanel;
+    static constexpr int state = 2 * stage;
+    static constexpr int turn = state + DK * DV * 2;  // results by stage, where the queries' place is too small
+    static constexpr int bytes = turn + (DV > DK ? 2 * (DV / 64) * kPanel : 0);
+    // one CTA per SM: all of tensor memory is its own
+    static constexpr int dynamic = (bytes < 120 * 1024 ? 120 * 1024 : bytes) + 1024;
+    static_assert(dynamic <= kMostShared, "shared memory");
+};
+
+template <int DK, int DV>
+struct SumLayout {
+    static constexpr int k = 0;
+    static constexpr int v = (DK / 64) * kPanel;
+    static constexpr int stage = v + (DV / 64) * kPanel;
+    static constexpr int stages = 3;
+    static constexpr int bytes = stages * stage;
+    static constexpr int dynamic = (bytes < 120 * 1024 ? 120 * 1024 : bytes) + 1024;
+    static_assert(dynamic <= kMostShared, "shared memory");
+};
+
+// l s as s + (l - 1) s where l is near one, so that many chunks do not add up l's rounding.
+struct Fade {
+    float whole, rest;
+};
+__device__ __forceinline__ Fade fade_of(double log_l) {
+    return log_l > -0.5 ? Fade{1.f, (float)expm1(log_l)} : Fade{(float)exp(log_l), 0.f};
+}
+__device__ __forceinline__ float faded(float s, Fade f) { return fmaf(s, f.rest, s * f.whole); }
+
+// Byte of column c in row r of a swizzled tile whose panels of 64 columns have `rows` rows.
+__device__ __forceinline__ uint32_t tile_byte(int r, int c, int rows) {
+    return (c >> 6) * (rows * 128) + r * 128 + ((((c >> 3) & 7) ^ (r & 7)) << 4) + (c & 7) * 2;
+}
+
+__device__ __forceinline__ float tile_value(const unsigned char *t, int r, int c, int rows) {
+    return __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(t + tile_byte(r, c, rows)));
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+__device__ __forceinline__ __nv_bfloat162 as_pair(uint32_t v) { return *reinterpret_cast<const __nv_bfloat162 *>(&v); }
+__device__ __forceinline__ uint32_t as_word(__nv_bfloat162 v) { return *reinterpret_cast<const uint32_t *>(&v); }
+
+// Barrier 1: the compute warps among themselves.
+__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kComputeWarps * 32) : "memory"); }
+// One segment of one head of one sequence.
+struct Line {
+    int start, count;  // rows of the sequence
+    int from, tokens;  // of the segment, in processing order
+    int last;          // the sequence's last segment
+    bool kept;         // has a slot in the state buffers
+    int64_t user;      // its state there
+    __device__ Line(const ChunkParams &cp, int segment, int h, int b) {
+        const MixParams &p = cp.p;
+        const Rows rows = rows_of(p.offsets, p.packed_tokens, p.length, b);
+        start = (int)rows.start;
+        count = (int)rows.count;
+        const int per_segment = cp.chunks * kChunk;
+        last = count > 0 ? (count - 1) / per_segment : 0;
+        from = segment * per_segment;
+        tokens = min(count - from, per_segment);
+        const int64_t slot = p.slots ? p.slots[b] : b;
+        kept = slot >= 0 && slot < p.state_slots;
+        user = (slot * p.heads + h) * (int64_t)p.dk * p.dv;
+    }
+    // first row of chunk c's tile; a tile in reverse ends at the last row not yet done
+    __device__ int first_row(int c, int reverse) const {
+        const int at = from + c * kChunk;
+        return start + (reverse ? count - at - kChunk : at);
+    }
+};
+
+__device__ __forceinline__ float *segment_state(const ChunkParams &cp, int64_t b, int h, int segment) {
+    return cp.segments + ((b * cp.p.heads + h) * cp.count + segment) * (int64_t)cp.p.dk * cp.p.dv;
+}
+
+// The rows of a chunk from the first on whose value holds an infinity or NaN, one by one: the
+// tensor cores' product with a masked score of zero would spread it to tokens before it, so
+// those get the product again without it, and the rest comes from here.  Rare and slow.
+template <int DK, int DV>
+__device__ __noinline__ void careful_rows(const unsigned char *sq, const unsigned char *sk, const unsigned char *sv,
+                                          const unsigned char *ss, const float *pw, int first, int last, int from, int reverse,
+                                          float inside, float before, void *out, int64_t ost, int dv, int out_f32) {
+    const int lane = threadIdx.x & 31;
+    for (int i = first + (threadIdx.x >> 5); i < last; i += kComputeWarps) {
+        if ((reverse ? kChunk - 1 - i : i) < from) continue;
+        float acc[DV / 32], state[DV / 32];
+#pragma unroll
+        for (int m = 0; m < DV / 32; m++) acc[m] = state[m] = 0.f;
+        for (int d = 0; d < DK; d++) {
+            const float q = tile_value(sq, i, d, kChunk);
+#pragma unroll
+            for (int m = 0; m < DV / 32; m++) state[m] = fmaf(q, tile_value(ss, d, lane + 32 * m, DK), state[m]);
+        }
+        const int j0 = reverse ? i : first, j1 = reverse ? last : i + 1;
+        for (int j = j0; j < j1; j++) {
+            float dot = 0.f;
+#pragma unroll
+            for (int m = 0; m < DK / 32; m++)
+                dot = fmaf(tile_value(sq, i, lane + 32 * m, kChunk), tile_value(sk, j, lane + 32 * m, kChunk), dot);
+            const float score = warp_sum(dot) * (inside * pw[reverse ? j - i : i - j]);
+#pragma unroll
+            for (int m = 0; m < DV / 32; m++) acc[m] = fmaf(score, tile_value(sv, j, lane + 32 * m, kChunk), acc[m]);
+        }
+        const float fade = before * pw[reverse ? kChunk - 1 - i : i + 1];
+#pragma unroll
+        for (int m = 0; m < DV / 32; m++) {
+            const int c = lane + 32 * m;
+            if (c >= dv) continue;
+            const float v = fmaf(fade, state[m], acc[m]);
+            if (out_f32)
+                static_cast<float *>(out)[i * ost + c] = v;
+            else
+                static_cast<__nv_bfloat16 *>(out)[i * ost + c] = __float2bfloat16_rn(v);
+        }
+    }
+}
+
+// W of 16 tile rows and 32 key columns: the weights w = w1 + w2 + w3 (bf16 terms) of this thread's rows, 2 (lane % 4),
+// 2 (lane % 4) + 1 and those 8 further on, times the keys.  k w1 = a + b and k w2 = c + d exactly (a product of two
+// 8-bit mantissas is its rounding and a bf16 remainder), so W = a + b + c + (d + k w3): only the last sum is rounded,
+// at 2^-25 of W.  Two terms are a and b + k w2, off by 2^-17.  Packed bf16 arithmetic: five (three) instructions for
+// two rows; terms cut out of the f32 product took twice as many.  ldmatrix turns the keys the way the tensor memory
+// wants them (a lane for each key column): one 2-byte load for each key had bound this step.
+template <int TERMS>
+__device__ __forceinline__ void make_weights(uint32_t keys, uint32_t unit, const uint32_t (&w)[3][2], uint32_t to, int term_columns) {
+#pragma unroll
+    for (int half = 0; half < 2; half++) {  // 16 key columns
+        uint32_t k4[4], t[TERMS][4];
+        load_blocks_transposed(keys + (unit ^ (half << 5)), k4);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const __nv_bfloat162 k = as_pair(k4[e]), w1 = as_pair(w[0][e >> 1]), w2 = as_pair(w[1][e >> 1]);
+            const __nv_bfloat162 a = __hmul2_rn(k, w1), b = __hfma2(k, w1, __hneg2(a));
+            t[0][e] = as_word(a);
+            if (TERMS == 2) {
+                t[1][e] = as_word(__hfma2(k, w2, b));
+            } else {
+                const __nv_bfloat162 c = __hmul2_rn(k, w2), d = __hfma2(k, w2, __hneg2(c));
+                t[1][e] = as_word(b);
+                t[2][e] = as_word(c);
+                t[3][e] = as_word(__hfma2(k, as_pair(w[2][e >> 1]), d));
+            }
+        }
+#pragma unroll
+        for (int term = 0; term < TERMS; term++)
+            tmem_store_blocks(to + (half << 20) + term * term_columns, t[term][0], t[term][1], t[term][2], t[term][3]);
+    }
+}
+
+// Loads the tiles that zeroing rows outside the sequence leaves: keys and values stand behind one another.
+template <int BYTES>
+__device__ __forceinline__ void clear_rows(unsigned char *tiles, int first, int end) {
+    for (int u = threadIdx.x; u < BYTES / 16; u += kComputeWarps * 32) {
+        const int r = (u >> 3) & (kChunk - 1);
+        if (r < first || r >= end) *reinterpret_cast<uint4 *>(tiles + u * 16) = make_uint4(0, 0, 0, 0);
+    }
+    fence_async_shared();
+    compute_sync();
+}
+
+// A segment's own sum: what its tokens leave of the state at its end, from a state of zero.  The weights reach to the
+// end of the segment, so that all chunks add up in tensor memory; four terms, as it is an f32 result.
+template <int DK, int DV>
+__global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant__ Maps maps,
+                                                          const __grid_constant__ ChunkParams cp) {
+    using L = SumLayout<DK, DV>;
+    constexpr int COLS = DV / kGroups;
+    constexpr int kBuffers = 3;                         // of W for half a chunk
+    constexpr uint32_t buffer_column[kBuffers] = {0, 128, 384};
+    extern __shared__ unsigned char raw[];
+    __shared__ __align__(8) uint64_t bars[2 * L::stages + 2 * kBuffers + 1];
+    __shared__ uint32_t tmem_word;
+    __shared__ int dead;
+    __shared__ float pw[kChunk + 1];  // update * l^n
+
+    const MixParams &p = cp.p;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int segment = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+    const Line line(cp, segment, h, b);
+    let_next_start();
+    if (segment > line.last || (segment == line.last && !p.s_out) || line.count == 0) return;
+    const int chunks = (line.tokens + kChunk - 1) / kChunk;
+
+    unsigned char *smem = raw + ((1024 - (shared_address(raw) & 1023)) & 1023);
+    const uint32_t base = shared_address(smem), bar0 = shared_address(bars);
+    const uint32_t full = bar0, free = bar0 + 8 * L::stages;                       // tiles have come; are used up
+    const uint32_t ready = bar0 + 16 * L::stages, used = ready + 8 * kBuffers;     // W is in place; is used up
+    const uint32_t all = used + 8 * kBuffers;
+    if (warp == 0) tmem_alloc(shared_address(&tmem_word), kTmemColumns);
+    if (tid == 0) {
+        for (int k = 0; k < 2 * L::stages + 2 * kBuffers + 1; k++)
+            barrier_init(bar0 + 8 * k, k >= 2 * L::stages && k < 2 * L::stages + kBuffers ? kComputeWarps : 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        dead = 0;
+    }
+    const float log_decay = p.log_decay[h];
+    if (tid <= kChunk) pw[tid] = (float)((tid ? exp((double)log_decay * tid) : 1.0) * p.update);
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const uint32_t tmem = tmem_word;
+    volatile int *gone = &dead;
+    // registers change hands by whole warpgroups
+    if (warp < kComputeWarps) {
+        more_registers<kComputeRegisters>();
+        const int group = warp >> 2, block = warp & 3, row = block * 32 + lane;
+        const uint32_t lanes = tmem + ((uint32_t)(block * 32) << 16);
+        const uint32_t keys = base + L::k + (block >> 1) * kPanel + ((lane & 7) + (lane >> 4) * 8) * 128;
+        const uint32_t unit = (((block & 1) * 4 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4;
+        for (int c = 0; c < chunks; c++) {
+            const int stage = c % L::stages, n = min(kChunk, line.tokens - c * kChunk);
+            const int first = p.reverse ? kChunk - n : 0, end = first + n;
+            // l^(tokens of the segment after this chunk)
+            const float later = expf(log_decay * (float)max(line.tokens - (c + 1) * kChunk, 0));
+            barrier_wait(full + 8 * stage, (c / L::stages) & 1, gone);
+            if (n < kChunk) clear_rows<L::stage>(smem + stage * L::stage, first, end);
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                const int i = 2 * c + half, buffer = i % kBuffers, r0 = half * 64 + group * 16 + 2 * (lane & 3);
+                uint32_t w[3][2];
+#pragma unroll
+                for (int pair = 0; pair < 2; pair++) {
+                    float f[2];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const int r = r0 + 8 * pair + e;
+                        f[e] = r >= first && r < end ? pw[p.reverse ? r + 1 - first : end - 1 - r] : 0.f;
+                        if (line.tokens - (c + 1) * kChunk > 0) f[e] *= later;
+                    }
+#pragma unroll
+                    for (int term = 0; term < 3; term++) {
+                        const uint32_t t = pack_bf16(f[0], f[1]);
+                        w[term][pair] = t;
+                        f[0] -= __uint_as_float(t << 16);
+                        f[1] -= __uint_as_float(t & 0xffff0000u);
+                    }
+                }
+                if (i >= kBuffers) {
+                    barrier_wait(used + 8 * buffer, (i / kBuffers - 1) & 1, gone);
+                    fence_after_sync();
+                }
+                if (row < DK)
+                    make_weights<4>(keys + stage * L::stage + (half * 4 + group) * 2048, unit, w,
+                                    lanes + buffer_column[buffer] + group * 8, 32);
+                tmem_store_wait();
+                fence_before_sync();
+                __syncwarp();
+                if (lane == 0) barrier_arrive(ready + 8 * buffer);
+            }
+        }
+        barrier_wait(all, 0, gone);
+        fence_after_sync();
+        if (row < DK) {
+            uint32_t x[COLS];
+            tmem_load(lanes + kZ + group * COLS, x);
+            if (row < p.dk) {
+                float *to = segment_state(cp, b, h, segment) + row * p.dv;
+#pragma unroll
+                for (int c = 0; c < COLS; c += 4)  // dv is a multiple of eight, the workspace aligned
+                    if (group * COLS + c < p.dv)
+                        *reinterpret_cast<uint4 *>(to + group * COLS + c) = make_uint4(x[c], x[c + 1], x[c + 2], x[c + 3]);
+            }
+        }
+    } else {
+        fewer_registers<kOtherRegisters>();
+        if (warp == kComputeWarps) {
+            if (lane == 0) {
+                const uint64_t values = matrix_desc(0, kPanel, 1024);
+                for (int i = 0; i < 2 * chunks; i++) {
+                    const int stage = (i >> 1) % L::stages, buffer = i % kBuffers;
+                    const uint64_t v = values + ((base + stage * L::stage + L::v + (i & 1) * 64 * 128) >> 4);
+                    barrier_wait(ready + 8 * buffer, (i / kBuffers) & 1, gone);
+                    fence_after_sync();
+                    const uint32_t w = tmem + buffer_column[buffer];
+#pragma unroll
+                    for (int term = 0; term < 4; term++)
+#pragma unroll
+                        for (int n = 0; n < 4; n++)
+                            mma_tensor(tmem + kZ, w + term * 32 + n * 8, v + (n * 2048 >> 4), mma_desc(DV, true),
+                                       i > 0 || term > 0 || n > 0);
+                    mma_commit(used + 8 * buffer);
+                    if (i & 1) mma_commit(free + 8 * stage);
+                }
+                mma_commit(all);
+            }
+        } else if (warp == kComputeWarps + 1) {
+            if (lane == 0) {
+                const int bb = p.offsets ? 0 : b;
+                int c = 0;
+                for (; c < chunks; c++) {
+                    const int stage = c % L::stages;
+                    if (c >= L::stages) barrier_wait(free + 8 * stage, (c / L::stages - 1) & 1, gone);
+                    if (dead) break;
+                    const uint32_t bar = full + 8 * stage, dst = base + stage * L::stage;
+                    const int t = line.first_row(c, p.reverse);
+                    barrier_expect(bar, L::stage);
+                    for (int n = 0; n < DK / 64; n++)
+                        tensor_load(dst + L::k + n * kPanel, &maps.k, bar, n * 64, h / p.k.per_head, t, bb);
+                    for (int n = 0; n < DV / 64; n++)
+                        tensor_load(dst + L::v + n * kPanel, &maps.v, bar, n * 64, h / p.v.per_head, t, bb);
+                }
+                for (int e = max(c - L::stages, 0); e < c; e++)  // no tile is on its way when the CTA ends
+                    for (int i = 0; i < 1 << 18 && !barrier_try(full + 8 * (e % L::stages), (e / L::stages) & 1); i++) {
+                    }
+            }
+        }
+    }
+    fence_before_sync();
+    __syncthreads();
+    if (tid == 0 && dead) atomicOr(p.err, 64);
+    if (warp == 0) tmem_free(tmem, kTmemColumns);
+}
+
+// The results of a segment, and (one segment) the final state.
+// TERMS: bf16 terms of the state update's weights.  Two (2^-17) where the state only goes on into results; four where
+// it is itself a result, in f32: then the weights of half a chunk fill the tensor memory that is left.
+template <int DK, int DV, int TERMS>
+__global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constant__ Maps maps,
+                                                            const __grid_constant__ ChunkParams cp) {
+    using L = Layout<DK, DV>;
+    constexpr int COLS = DV / kGroups;  // state and result columns of one thread
+    constexpr int HALVES = TERMS == 4 ? 2 : 1, kTermColumns = kChunk / 2 / HALVES;
+    extern __shared__ unsigned char raw[];
+    __shared__ __align__(8) uint64_t bars[14];
+    __shared__ uint32_t tmem_word;
+    __shared__ int dead, first_odd, odd_values;
+    __shared__ int careful_at[2];                              // by stage: 0, or which careful chunk it is
+    __shared__ float pw[kChunk + 1];                           // l^n
+    __shared__ __align__(16) uint32_t weight[3][kChunk / 2];   // of pairs of tile rows, as three bf16 terms
+    // l^n along the columns of a block of scores away from the diagonal, and on it (there times l^-n of the
+    // rows or columns, where that stays in range)
+    __shared__ __align__(16) float column[32], diagonal[32];
+
+    const MixParams &p = cp.p;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int segment = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+    const Line line(cp, segment, h, b);
+    if (segment > line.last) return;
+    const int chunks = (line.tokens + kChunk - 1) / kChunk;
+    if (line.count == 0) {  // an empty sequence: its state passes through (with segments: before this kernel)
+        if (cp.count == 1 && p.s_out && line.kept)
+            for (int e = tid; e < p.dk * p.dv; e += kThreads) {
+                const int64_t at = line.user + (e / p.dv) * p.state_k + (e % p.dv) * p.state_v;
+                p.s_out[at] = p.s_in ? p.s_in[at] : 0.f;
+            }
+        return;
+    }
+
+    unsigned char *smem = raw + ((1024 - (shared_address(raw) & 1023)) & 1023);
+    const uint32_t base = shared_address(smem);
+    const uint32_t bar0 = shared_address(bars);
+    // by stage: tiles have come; every compute warp is done with a chunk
+    const uint32_t full = bar0, done = bar0 + 16;
+    // products that have come out
+    const uint32_t bar_x = bar0 + 32, bar_y = bar0 + 40, bar_w = bar0 + 48, bar_o = bar0 + 56, bar_z = bar0 + 64,
+                   bar_again = bar0 + 72;
+    // operands that every warp concerned has put in place
+    const uint32_t w0_ready = bar0 + 80, w1_ready = bar0 + 88, p_ready = bar0 + 96, v_ready = bar0 + 104;
+    if (warp == 0) tmem_alloc(shared_address(&tmem_word), kTmemColumns);
+    if (tid == 0) {
+        for (int k = 0; k < 14; k++)
+            barrier_init(bar0 + 8 * k, k == 12 ? kComputeWarps + 2 : k == 2 || k == 3 || k >= 10 ? kComputeWarps : 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        dead = odd_values = 0;
+        careful_at[0] = careful_at[1] = 0;
+    }
+    const float log_decay = p.log_decay[h];
+    if (tid <= kChunk) {
+        const double l = tid ? exp((double)log_decay * tid) : 1.0;
+        pw[tid] = (float)l;
+        if (tid < 32) {
+            column[p.reverse ? tid : 31 - tid] = (float)l;
+            diagonal[tid] = (float)(p.reverse ? l : 1.0 / l);
+        }
+    }
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const uint32_t tmem = tmem_word;
+    unsigned char *state_tile = smem + L::state;
+    volatile int *gone = &dead;
+    // registers change hands by whole warpgroups
+    if (warp < kComputeWarps) {
+        more_registers<kComputeRegisters>();
+        // ---- the other warps
+        const int group = warp >> 2, block = warp & 3;  // share of the columns; block of 32 rows (tensor memory lanes)
+        const int row = block * 32 + lane;
+        const bool state_row = row < DK;
+        const uint32_t lanes = tmem + ((uint32_t)(block * 32) << 16);
+        const float inside = p.update * p.out;
+        auto arrive = [&](uint32_t bar) {
+            fence_before_sync();
+            __syncwarp();
+            if (lane == 0) barrier_arrive(bar);
+        };
+
+        // the state: row `row`, columns from group * COLS
+        float s[COLS];
+        auto publish_state = [&] {
+            if (state_row) {
+#pragma unroll
+                for (int c = 0; c < COLS; c += 8) {
+                    uint4 v;
+                    v.x = pack_bf16(s[c], s[c + 1]), v.y = pack_bf16(s[c + 2], s[c + 3]);
+                    v.z = pack_bf16(s[c + 4], s[c + 5]), v.w = pack_bf16(s[c + 6], s[c + 7]);
+                    *reinterpret_cast<uint4 *>(state_tile + tile_byte(row, group * COLS + c, DK)) = v;
+                }
+            }
+            fence_async_shared();
+        };
+        {
+            wait_for_previous();
+            const float *in = cp.count > 1 ? segment_state(cp, b, h, segment) : p.s_in && line.kept ? p.s_in + line.user : nullptr;
+            const int64_t in_k = cp.count > 1 ? p.dv : p.state_k, in_v = cp.count > 1 ? 1 : p.state_v;
+            const bool wide = in && in_v == 1 && (p.dv & 3) == 0 && (reinterpret_cast<uintptr_t>(in) & 15) == 0;
+#pragma unroll
+            for (int c = 0; c < COLS; c += 4) {
+                const int col = group * COLS + c;
+                if (wide && row < p.dk && col < p.dv) {
+                    const float4 v = *reinterpret_cast<const float4 *>(in + row * in_k + col);
+                    s[c] = v.x, s[c + 1] = v.y, s[c + 2] = v.z, s[c + 3] = v.w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        s[c + e] = in && row < p.dk && col + e < p.dv ? in[row * in_k + (col + e) * in_v] : 0.f;
+                }
+            }
+            publish_state();
+            arrive(done + 8);
+        }
+
+        int powers_of = 0;
+        Fade keep{1.f, 0.f};
+        // blocks of keys as ldmatrix reads them: lane i names row i % 8 + 8 (i / 16) and 8 columns, i / 8 % 2
+        const uint32_t keys = base + L::k + (block >> 1) * kPanel + ((lane & 7) + (lane >> 4) * 8) * 128;
+        const uint32_t unit = (((block & 1) * 4 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4;
+        const bool gentle = log_decay > -2.5f;  // l^-31 is in range
+        for (int c = 0; c < chunks; c++) {
+            const int parity = c & 1;
+            const int n = min(kChunk, line.tokens - c * kChunk);
+            const int first = p.reverse ? kChunk - n : 0, end = first + n;  // valid tile rows
+            unsigned char *tile = smem + (c & 1) * L::stage;
+            if (n != powers_of) {  // the first chunk, and a last one that is shorter
+                powers_of = n;
+                keep = fade_of((double)log_decay * n);
+                compute_sync();
+                if (tid < kChunk / 2) {
+                    // tile row r: update * l^(rows after it), reverse: l^(rows before it and itself)
+                    float w[2];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const int r = 2 * tid + e;
+                        w[e] = r >= first && r < end ? p.update * pw[p.reverse ? r + 1 - first : end - 1 - r] : 0.f;
+                    }
+#pragma unroll
+                    for (int term = 0; term < 3; term++) {
+                        const uint32_t t = pack_bf16(w[0], w[1]);
+                        weight[term][tid] = t;
+                        w[0] -= __uint_as_float(t << 16);
+                        w[1] -= __uint_as_float(t & 0xffff0000u);
+                    }
+                }
+                compute_sync();
+            }
+            barrier_wait(full + 8 * (c & 1), (c >> 1) & 1, gone);
+            if (n < kChunk) clear_rows<L::stage - L::k>(tile + L::k, first, end);
+
+            // W of 16 rows
+            auto weigh = [&](int at, int column) {
+                if (!state_row) return;
+                uint32_t w[3][2];
+#pragma unroll
+                for (int term = 0; term < (TERMS == 2 ? 2 : 3); term++) {
+                    w[term][0] = weight[term][at * 8 + (lane & 3)];
+                    w[term][1] = weight[term][at * 8 + (lane & 3) + 4];
+                }
+                make_weights<TERMS>(keys + (c & 1) * L::stage + at * 2048, unit, w, lanes + kW + column, kTermColumns);
+            };
+            if (HALVES == 2) {
+                weigh(group, group * 8);
+            } else {
+                weigh(group, group * 8);
+                weigh(4 + group, 32 + group * 8);
+            }
+            tmem_store_wait();
+            arrive(w0_ready);
+
+            // scores -> P in place: a block of 32 columns leaves 16 columns of bf16 pairs behind
+            barrier_wait(bar_x, parity, gone);
+            fence_after_sync();
+            {
+                const uint32_t at = lanes + kX + group * 32;
+                uint32_t packed[16];
+                if (p.reverse ? group < block : group > block) {  // all of it lies ahead
+#pragma unroll
+                    for (int j = 0; j < 16; j++) packed[j] = 0;
+                } else {
+                    uint32_t x[32];
+                    tmem_load(at, x);
+                    const bool on = group == block;
+                    if (on && !gentle) {
+#pragma unroll
+                        for (int j = 0; j < 32; j++) {
+                            const int gap = p.reverse ? j - lane : lane - j;
+                            x[j] = gap >= 0 ? __float_as_uint(__uint_as_float(x[j]) * (inside * pw[max(gap, 0)])) : 0;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 16; j++) packed[j] = pack_bf16(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]));
+                    } else {
+                        const float f = inside * (on ? (p.reverse ? 1.f / pw[lane] : pw[lane])
+                                                     : pw[p.reverse ? group * 32 - row : row - group * 32 - 31]);
+                        const float *along = on ? diagonal : column;
+                        const uint64_t ff = pair_of(f, f);
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            const float4 w = *reinterpret_cast<const float4 *>(along + j);
+                            float y[4];
+                            split_pair(mul_pair(pair_of(__uint_as_float(x[j]), __uint_as_float(x[j + 1])),
+                                                mul_pair(ff, pair_of(w.x, w.y))), y[0], y[1]);
+                            split_pair(mul_pair(pair_of(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])),
+                                                mul_pair(ff, pair_of(w.z, w.w))), y[2], y[3]);
+                            packed[j / 2] = pack_bf16(y[0], y[1]);
+                            packed[j / 2 + 1] = pack_bf16(y[2], y[3]);
+                        }
+                        if (on) {  // columns ahead of this row: a shift by 0, 16 or 32 bits leaves none, one or both
+                            if (p.reverse) {
+#pragma unroll
+                                for (int j = 0; j < 16; j++) packed[j] &= __funnelshift_rc(0, ~0u, max(32 * j + 32 - 16 * lane, 0));
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 16; j++) packed[j] &= __funnelshift_lc(~0u, 0, max(16 * lane + 16 - 32 * j, 0));
+                            }
+                        }
+                    }
+                }
+                tmem_store(at, packed);
+            }
+            // the state's part of the result, faded by row; the product inside the chunk adds to it
+            barrier_wait(bar_y, parity, gone);
+            fence_after_sync();
+            {
+                const float fade = p.out * pw[p.reverse ? kChunk - 1 - row : row + 1];
+                uint32_t x[COLS];
+                tmem_load(lanes + kY + group * COLS, x);
+#pragma unroll
+                for (int j = 0; j < COLS; j += 2) {
+                    float a, b;
+                    split_pair(mul_pair(pair_of(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), pair_of(fade, fade)), a, b);
+                    x[j] = __float_as_uint(a), x[j + 1] = __float_as_uint(b);
+                }
+                tmem_store(lanes + kY + group * COLS, x);
+            }
+            tmem_store_wait();
+            arrive(p_ready);
+
+            if (HALVES == 2) {  // the second half's weights, where the first half's were
+                barrier_wait(bar_w, parity, gone);
+                fence_after_sync();
+                weigh(4 + group, group * 8);
+                tmem_store_wait();
+                arrive(w1_ready);
+            }
+            // S <- l^rows S + update, while the product inside the chunk goes on
+            auto step_state = [&] {
+                barrier_wait(bar_z, parity, gone);
+                fence_after_sync();
+                if (state_row) {
+                    uint32_t x[COLS];
+                    tmem_load(lanes + kZ + group * COLS, x);
+                    const uint64_t whole = pair_of(keep.whole, keep.whole), rest = pair_of(keep.rest, keep.rest);
+#pragma unroll
+                    for (int j = 0; j < COLS; j += 2) {
+                        const uint64_t old = pair_of(s[j], s[j + 1]);
+                        split_pair(add_pair(fma_pair(old, rest, mul_pair(old, whole)),
+                                            pair_of(__uint_as_float(x[j]), __uint_as_float(x[j + 1]))), s[j], s[j + 1]);
+                    }
+                }
+            };
+            if (HALVES == 1) step_state();
+
+            barrier_wait(bar_o, parity, gone);
+            fence_after_sync();
+            {
+                const bool careful = *(volatile int *)&careful_at[c & 1];
+                const bool sent = n == kChunk && !careful && !cp.out_f32;  // whole chunks leave as tiles
+                const int64_t out_at =
+                    sent ? 0 : (p.offsets ? 0 : b * p.osb) + h * p.osh + line.first_row(c, p.reverse) * p.ost;
+                int stop = kChunk;  // rows from here on, in processing order, are careful_rows' own
+                if (careful) {
+                    const unsigned char *sk = tile + L::k;
+                    unsigned char *sv = tile + L::v;
+                    barrier_wait(bar_z, parity, gone);
+                    fence_after_sync();
+                    if (tid == 0) first_odd = kChunk;
+                    compute_sync();
+                    for (int u = tid; u < kChunk * DV; u += kComputeWarps * 32) {
+                        const int r = u / DV;
+                        const float v = tile_value(sv, r, u % DV, kChunk);
+                        if (!(fabsf(v) <= 3.4e38f)) atomicMin(&first_odd, p.reverse ? kChunk - 1 - r : r);
+                    }
+                    compute_sync();
+                    stop = *(volatile int *)&first_odd;
+                    void *o = cp.out_f32 ? (void *)(static_cast<float *>(p.o) + out_at)
+                                         : (void *)(static_cast<__nv_bfloat16 *>(p.o) + out_at);
+                    careful_rows<DK, DV>(tile + L::q, sk, sv, state_tile, pw, first, end, stop, p.reverse, inside, p.out,
+                                         o, p.ost, p.dv, cp.out_f32);
+                    compute_sync();
+                    for (int u = tid; u < kChunk * DV; u += kComputeWarps * 32) {
+                        const int r = u / DV, col = u % DV;
+                        if (!(fabsf(tile_value(sv, r, col, kChunk)) <= 3.4e38f))
+                            *reinterpret_cast<__nv_bfloat16 *>(sv + tile_byte(r, col, kChunk)) = __float2bfloat16_rn(0.f);
+                    }
+                    fence_async_shared();
+                    arrive(v_ready);
+                    barrier_wait(bar_again, (careful_at[c & 1] - 1) & 1, gone);
+                    fence_after_sync();
+                }
+                const int low = p.reverse ? max(first, kChunk - stop) : first, high = p.reverse ? end : min(end, stop);
+                uint32_t y[COLS];
+                tmem_load(lanes + kY + group * COLS, y);
+                if (cp.out_f32) {
+                    float *o = static_cast<float *>(p.o) + out_at + row * p.ost;
+                    if (row >= low && row < high) {
+#pragma unroll
+                        for (int k = 0; k < COLS; k += 4)
+                            if (group * COLS + k < p.dv)
+                                *reinterpret_cast<uint4 *>(o + group * COLS + k) = make_uint4(y[k], y[k + 1], y[k + 2], y[k + 3]);
+                    }
+                } else {
+                    // through shared memory, in the queries' place or one of its own
+                    unsigned char *turn = smem + (DV > DK ? L::turn + (c & 1) * (DV / 64) * kPanel : (c & 1) * L::stage + L::q);
+#pragma unroll
+                    for (int k = 0; k < COLS; k += 8) {
+                        uint32_t v[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            v[e] = pack_bf16(__uint_as_float(y[k + 2 * e]), __uint_as_float(y[k + 2 * e + 1]));
+                        *reinterpret_cast<uint4 *>(turn + tile_byte(row, group * COLS + k, kChunk)) =
+                            make_uint4(v[0], v[1], v[2], v[3]);
+                    }
+                    if (!sent) {  // row pieces of the warp's own rows
+                        __syncwarp();
+                        constexpr int PER = COLS / 8;  // 16-byte pieces of a row
+                        __nv_bfloat16 *o = static_cast<__nv_bfloat16 *>(p.o) + out_at;
+                        for (int u = 0; u < PER; u++) {
+                            const int r = block * 32 + u * (32 / PER) + lane / PER, col = group * COLS + (lane % PER) * 8;
+                            if (r >= low && r < high && col < p.dv)
+                                *reinterpret_cast<uint4 *>(o + r * p.ost + col) =
+                                    *reinterpret_cast<const uint4 *>(turn + tile_byte(r, col, kChunk));
+                        }
+                    }
+                }
+            }
+            if (HALVES == 2) step_state();
+            publish_state();
+            arrive(done + 8 * (c & 1));
+        }
+        if (TERMS == 4 && !dead && p.s_out && line.kept && row < p.dk) {
+            float *to = p.s_out + line.user + row * p.state_k;
+            const bool wide = p.state_v == 1 && (p.dv & 3) == 0 && (reinterpret_cast<uintptr_t>(to) & 15) == 0;
+#pragma unroll
+            for (int c = 0; c < COLS; c += 4) {
+                const int col = group * COLS + c;
+                if (wide && col < p.dv) {
+                    *reinterpret_cast<float4 *>(to + col) = make_float4(s[c], s[c + 1], s[c + 2], s[c + 3]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (col + e < p.dv) to[(col + e) * p.state_v] = s[c + e];
+                }
+            }
+        }
+    } else {
+        fewer_registers<kOtherRegisters>();
+        if (warp == kComputeWarps) {
+            // ---- one thread issues the products
+            if (lane == 0) {
+                const uint64_t by_k = matrix_desc(0, 16, 1024);                 // contiguous axis summed over
+                const uint64_t values = matrix_desc(0, kPanel, 1024), state = matrix_desc(base + L::state, DK * 128, 1024);
+                auto scores = [&](int c) {
+                    barrier_wait(full + 8 * (c & 1), (c >> 1) & 1, gone);
+                    const uint64_t q = by_k + ((base + (c & 1) * L::stage + L::q) >> 4);
+                    const uint64_t k = by_k + ((base + (c & 1) * L::stage + L::k) >> 4);
+#pragma unroll
+                    for (int n = 0; n < DK / 16; n++) {
+                        const uint32_t at = ((n >> 2) * kPanel + (n & 3) * 32) >> 4;
+                        mma_shared(tmem + kX, q + at, k + at, mma_desc(128, false), n > 0);
+                    }
+                    mma_commit(bar_x);
+                };
+                scores(0);
+                for (int c = 0; c < chunks; c++) {
+                    const int parity = c & 1;
+                    const uint32_t tile_at = base + (c & 1) * L::stage;
+                    const uint64_t v = values + ((tile_at + L::v) >> 4);
+                    auto update = [&](int half) {
+#pragma unroll
+                        for (int term = 0; term < TERMS; term++)
+#pragma unroll
+                            for (int n = 0; n < 8 / HALVES; n++)
+                                mma_tensor(tmem + kZ, tmem + kW + term * kTermColumns + n * 8, v + ((half * 64 + n * 16) * 128 >> 4),
+                                           mma_desc(DV, true), half > 0 || term > 0 || n > 0);
+                    };
+                    auto inside_product = [&] {
+#pragma unroll
+                        for (int n = 0; n < 8; n++)
+                            mma_tensor(tmem + kY, tmem + kX + (n >> 1) * 32 + (n & 1) * 8, v + (n * 2048 >> 4), mma_desc(DV, true),
+                                       true);
+                    };
+                    // c = 0: the state that enters is in place (every compute warp is done with chunk -1, stage 1)
+                    barrier_wait(done + 8 * ((c + 1) & 1), (c >> 1) & 1, gone);
+                    fence_after_sync();
+                    const uint64_t q = by_k + ((tile_at + L::q) >> 4);
+#pragma unroll
+                    for (int n = 0; n < DK / 16; n++)
+                        mma_shared(tmem + kY, q + (((n >> 2) * kPanel + (n & 3) * 32) >> 4), state + (n * 2048 >> 4),
+                                   mma_desc(DV, true), n > 0);
+                    mma_commit(bar_y);
+                    barrier_wait(w0_ready, parity, gone);
+                    fence_after_sync();
+                    update(0);
+                    mma_commit(HALVES == 2 ? bar_w : bar_z);
+                    barrier_wait(p_ready, parity, gone);
+                    fence_after_sync();
+                    const int careful = *(volatile int *)&careful_at[c & 1];
+                    if (!careful) inside_product();
+                    mma_commit(bar_o);
+                    if (HALVES == 2) {
+                        barrier_wait(w1_ready, parity, gone);
+                        fence_after_sync();
+                        update(1);
+                        mma_commit(bar_z);
+                    }
+                    if (careful) {
+                        barrier_wait(v_ready, (careful - 1) & 1, gone);
+                        fence_after_sync();
+                        inside_product();
+                        mma_commit(bar_again);
+                    }
+                    if (c + 1 < chunks) scores(c + 1);
+                }
+            }
+        } else if (warp == kComputeWarps + 1) {
+            // ---- one thread fetches the tiles and sends the results away
+            if (lane == 0) {
+                const int bb = p.offsets ? 0 : b;
+                // the results of chunk c stand in shared memory, unless its threads wrote them themselves
+                auto finish = [&](int c) {
+                    barrier_wait(done + 8 * (c & 1), ((c >> 1) + (c & 1)) & 1, gone);
+                    if (cp.out_f32 || dead || *(volatile int *)&careful_at[c & 1] || line.tokens - c * kChunk < kChunk) return;
+                    const uint32_t src = base + (DV > DK ? L::turn + (c & 1) * (DV / 64) * kPanel : (c & 1) * L::stage + L::q);
+                    const int t = line.first_row(c, p.reverse);
+                    for (int n = 0; n < DV / 64; n++)
+                        if (n * 64 < p.dv) tensor_store(&maps.o, src + n * kPanel, n * 64, h, t, bb);
+                    tensor_store_read();
+                };
+                int c = 0;
+                for (; c < chunks; c++) {
+                    if (c >= 2) finish(c - 2);
+                    if (dead) break;
+                    const uint32_t bar = full + 8 * (c & 1), dst = base + (c & 1) * L::stage;
+                    const int t = line.first_row(c, p.reverse);
+                    barrier_expect(bar, L::stage);
+                    for (int n = 0; n < DK / 64; n++)
+                        tensor_load(dst + L::k + n * kPanel, &maps.k, bar, n * 64, h / p.k.per_head, t, bb);
+                    for (int n = 0; n < DK / 64; n++)
+                        tensor_load(dst + L::q + n * kPanel, &maps.q, bar, n * 64, h / p.q.per_head, t, bb);
+                    for (int n = 0; n < DV / 64; n++)
+                        tensor_load(dst + L::v + n * kPanel, &maps.v, bar, n * 64, h / p.v.per_head, t, bb);
+                }
+                if (c == chunks) {
+                    if (c > 1) finish(c - 2);
+                    finish(c - 1);
+                }
+                // no tile is on its way when the CTA ends
+                for (int e = max(c - 2, 0); e < c; e++)
+                    for (int i = 0; i < 1 << 18 && !barrier_try(full + 8 * (e & 1), (e >> 1) & 1); i++) {
+                    }
+            }
+        } else {
+            // ---- two warps look for infinities and NaN among the values
+            const int which = warp - kComputeWarps - 2;  // half of the rows
+            int careful_chunks = 0;
+            for (int c = 0; c < chunks; c++) {
+                const int n = min(kChunk, line.tokens - c * kChunk);
+                const int first = p.reverse ? kChunk - n : 0, end = first + n;
+                const unsigned char *sv = smem + (c & 1) * L::stage + L::v + which * 64 * 128 + lane * 16;
+                barrier_wait(full + 8 * (c & 1), (c >> 1) & 1, gone);
+                uint32_t odd = 0;
+                for (int panel = 0; panel < DV / 64; panel++)
+#pragma unroll 4
+                    for (int u = 0; u < 16; u++) {  // four rows at a time
+                        const uint4 w = *reinterpret_cast<const uint4 *>(sv + panel * kPanel + u * 512);
+                        const int r = which * 64 + u * 4 + (lane >> 3);
+                        uint32_t here = (w.x & 0x7f807f80u) + 0x00800080u;
+                        here |= (w.y & 0x7f807f80u) + 0x00800080u;
+                        here |= (w.z & 0x7f807f80u) + 0x00800080u;
+                        here |= (w.w & 0x7f807f80u) + 0x00800080u;
+                        if (r >= first && r < end) odd |= here;
+                    }
+                const bool any = __any_sync(~0u, odd & 0x80008000u);
+                // the first of them tells what both found
+                if (lane == 0 && any) atomicOr(&odd_values, 1);
+                asm volatile("bar.sync 2, 64;" ::: "memory");
+                if (which == 0 && lane == 0) {
+                    const bool found = *(volatile int *)&odd_values;
+                    careful_chunks += found;
+                    careful_at[c & 1] = found ? careful_chunks : 0;
+                    odd_values = 0;
+                }
+                asm volatile("bar.sync 2, 64;" ::: "memory");
+                if (c > 0) barrier_wait(p_ready, (c - 1) & 1, gone);  // one arrival a chunk
+                __syncwarp();
+                if (lane == 0) barrier_arrive(p_ready);
+            }
+        }
+    }
+    fence_before_sync();
+    __syncthreads();
+    if (tid == 0 && dead) atomicOr(p.err, 64);
+    if (warp == 0) tmem_free(tmem, kTmemColumns);
+}
+
+// Turns the segments' own sums into the states that enter them, in order, and leaves the final state.
+// Four elements to a thread (dv is a multiple of eight), eight loads in flight.
+__global__ void __launch_bounds__(128) enter_kernel(const __grid_constant__ ChunkParams cp) {
+    constexpr int AHEAD = 8;
+    __shared__ Fade fades[2];
+    const MixParams &p = cp.p;
+    const int h = blockIdx.y, b = blockIdx.z, e = (blockIdx.x * 128 + threadIdx.x) * 4, n = p.dk * p.dv;
+    const Line line(cp, 0, h, b);
+    const int per_segment = cp.chunks * kChunk, last = line.last;
+    if (threadIdx.x < 2)
+        fades[threadIdx.x] = fade_of((double)p.log_decay[h] * (threadIdx.x ? line.count - last * per_segment : per_segment));
+    let_next_start();
+    __syncthreads();
+    if (e >= n) return;
+    const Fade keep = fades[0], keep_last = fades[1];
+    const int64_t user = line.user + (e / p.dv) * p.state_k + (e % p.dv) * p.state_v;
+    wait_for_previous();
+    float s[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) s[i] = p.s_in && line.kept ? p.s_in[user + i * p.state_v] : 0.f;
+    float4 *at = reinterpret_cast<float4 *>(segment_state(cp, b, h, 0) + e);
+    const int step = n / 4;
+    const int sums = p.s_out && line.count > 0 ? last + 1 : last;  // the last segment's is there if someone wants it
+    for (int k0 = 0; k0 <= last; k0 += AHEAD) {
+        float4 sum[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) sum[k] = k0 + k < sums ? at[(int64_t)(k0 + k) * step] : make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++)
+            if (k0 + k <= last) {
+                at[(int64_t)(k0 + k) * step] = make_float4(s[0], s[1], s[2], s[3]);
+                const Fade f = k0 + k < last ? keep : keep_last;
+                s[0] = faded(s[0], f) + sum[k].x, s[1] = faded(s[1], f) + sum[k].y;
+                s[2] = faded(s[2], f) + sum[k].z, s[3] = faded(s[3], f) + sum[k].w;
+            }
+    }
+    if (p.s_out && line.kept) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) p.s_out[user + i * p.state_v] = s[i];
+    }
+}
+
+using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                            const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                            CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+Encode encoder() {
+    static const Encode fn = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult got;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &got) != cudaSuccess) f = nullptr;
+        return reinterpret_cast<Encode>(f);
+    }();
+    return fn;
+}
+
+// [dim, heads, tokens, batch] with boxes of 64 x 1 x 128 x 1
+void encode(CUtensorMap &map, const MixOperand &t, const MixParams &p, int dim) {
+    const int64_t heads = (p.heads + t.per_head - 1) / t.per_head;
+    const int64_t tokens = p.offsets ? p.packed_tokens : p.length, batch = p.offsets ? 1 : p.batch;
+    const cuuint64_t size[4] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)tokens, (cuuint64_t)batch};
+    const cuuint64_t stride[3] = {(cuuint64_t)t.sh * 2, (cuuint64_t)t.st * 2, (cuuint64_t)(p.offsets ? t.st * 2 : t.sb * 2)};
+    const cuuint32_t box[4] = {64, 1, kChunk, 1}, step[4] = {1, 1, 1, 1};
+    const CUresult r = encoder()(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(t.p), size, stride, box, step,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) fail_runtime("tensor map encoding failed: error " + std::to_string((int)r));
+}
+
+bool loadable(const MixOperand &t, int dim) {
+    const int64_t widest = int64_t(1) << 38;  // strides stay below 2^40 bytes
+    return dim % 8 == 0 && (reinterpret_cast<uintptr_t>(t.p) & 15) == 0 && t.sb % 8 == 0 && t.st % 8 == 0 &&
+           t.sh % 8 == 0 && t.sb < widest && t.st < widest && t.sh < widest;
+}
+
+// after: the kernel may start while the one before it ends (it waits for it where it reads its results)
+template <typename Kernel, typename... Args>
+cudaError_t launch(Kernel *kernel, dim3 grid, int threads, int shared, bool after, cudaStream_t s, const Args &...args) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = shared;
+    config.stream = s;
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute;
+    config.numAttrs = after ? 1 : 0;
+    if (shared) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
+        if (e != cudaSuccess) return e;
+    }
+    before_launch();
+    return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
+template <int DK, int DV>
+cudaError_t launch_all(const Maps &maps, const ChunkParams &cp, cudaStream_t s) {
+    const dim3 grid(cp.count, cp.p.heads, (unsigned)cp.p.batch);
+    if (cp.count == 1)  // the state itself is a result (and, wanted or not, it makes the same results)
+        return launch(chunk_kernel<DK, DV, 4>, grid, kThreads, Layout<DK, DV>::dynamic, false, s, maps, cp);
+    cudaError_t e = launch(sum_kernel<DK, DV>, grid, kThreads, SumLayout<DK, DV>::dynamic, false, s, maps, cp);
+    if (e != cudaSuccess) return e;
+    const dim3 elements((cp.p.dk * cp.p.dv + 511) / 512, cp.p.heads, (unsigned)cp.p.batch);
+    e = launch(enter_kernel, elements, 128, 0, true, s, cp);
+    if (e != cudaSuccess) return e;
+    return launch(chunk_kernel<DK, DV, 2>, grid, kThreads, Layout<DK, DV>::dynamic, true, s, maps, cp);
+}
+
+}  // namespace
+
+Segments segments_of(int64_t length, int64_t batch, int64_t heads) {
+    const int64_t chunks = (length + kChunk - 1) / kChunk, lines = batch * heads;
+    // microseconds: waves of CTAs, each with its start and its chunks.  One segment: 3.5 a chunk (four terms);
+    // more: 3.1 and 1.6 for the pass before it, twice the start, and the kernel between the two.
+    Segments best{1, (int)chunks};
+    double least = 0;
+    for (int64_t want = 1; want <= std::min<int64_t>(chunks, 64); want++) {
+        const int64_t per = (chunks + want - 1) / want, count = (chunks + per - 1) / per;
+        if (count > 1 && lines * count > 8 * kSms) break;
+        const double waves = (double)((lines * count + kSms - 1) / kSms);
+        const double time = count == 1 ? waves * (3.5 * per + 5) : waves * (4.7 * per + 12) + 10;
+        if (want == 1 || time < least) {
+            least = time;
+            best = {(int)count, (int)per};
+        }
+    }
+    return best;
+}
+
+bool chunked_tc_takes(const MixParams &p, Element e, bool out_f32) {
+    if (e != Element::BF16 || p.dk > 128 || p.dv > 128 || p.length < 2) return false;
+    if (!loadable(p.q, p.dk) || !loadable(p.k, p.dk) || !loadable(p.v, p.dv)) return false;
+    const int64_t tokens = p.offsets ? p.packed_tokens : p.length;
+    if (tokens == 0 || std::max(tokens, p.length) > int64_t(1) << 30) return false;  // rows are counted in 32 bits
+    const bool stores = out_f32 ? (reinterpret_cast<uintptr_t>(p.o) & 15) == 0 && p.osb % 4 == 0 && p.ost % 4 == 0 && p.osh % 4 == 0
+                                : loadable({p.o, p.osb, p.ost, p.osh, 1}, p.dv);
+    return stores && encoder();
+}
+
+cudaError_t launch_chunked_tc(const MixParams &p, bool out_f32, float *segments, cudaStream_t s) {
+    Maps maps;
+    encode(maps.q, p.q, p, p.dk);
+    encode(maps.k, p.k, p, p.dk);
+    encode(maps.v, p.v, p, p.dv);
+    if (!out_f32) encode(maps.o, {p.o, p.osb, p.ost, p.osh, 1}, p, p.dv);
+    ChunkParams cp{};
+    cp.p = p;
+    cp.segments = segments;
+    const Segments g = segments_of(p.length, p.batch, p.heads);
+    cp.count = g.count;
+    cp.chunks = g.chunks;
+    cp.out_f32 = out_f32;
+    if (p.dk <= 64) return p.dv <= 64 ? launch_all<64, 64>(maps, cp, s) : launch_all<64, 128>(maps, cp, s);
+    return p.dv <= 64 ? launch_all<128, 64>(maps, cp, s) : launch_all<128, 128>(maps, cp, s);
+}
+
+}  // namespace b200fft

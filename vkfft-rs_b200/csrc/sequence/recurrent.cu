@@ -47,9 +47,11 @@ __global__ void __launch_bounds__(kThreads) recurrent_kernel(MixParams p) {
                               : 0.f;
         }
     }
-    // l in two parts: rounded to one, slow decays would be off by up to 2^-25 a token, always to the same side
+    // l S as S + (l - 1) S where l is near one: rounded to f32, such an l would be off by up to
+    // 2^-25 a token, always to the same side
     const float log_decay = p.log_decay[h];
-    const float l = expf(log_decay), l_rest = log_decay > -0.5f ? expm1f(log_decay) - (l - 1.f) : 0.f;
+    const bool slow = log_decay > -0.5f;
+    const float l = slow ? 1.f : expf(log_decay), l_rest = slow ? expm1f(log_decay) : 0.f;
     const T *q = static_cast<const T *>(p.q.p) + (p.offsets ? 0 : b * p.q.sb) + (h / p.q.per_head) * p.q.sh;
     const T *k = static_cast<const T *>(p.k.p) + (p.offsets ? 0 : b * p.k.sb) + (h / p.k.per_head) * p.k.sh;
     const T *v = static_cast<const T *>(p.v.p) + (p.offsets ? 0 : b * p.v.sb) + (h / p.v.per_head) * p.v.sh;

@@ -151,11 +151,20 @@ LinearAttention LinearAttention::from_c(const b200fft_linear_attention_config &c
     return a;
 }
 
-size_t LinearAttention::workspace() const { return 0; }
+size_t LinearAttention::segment_bytes() const {
+    if (length < 2) return 0;
+    const Segments g = segments_of(length, batch, heads);
+    return g.count > 1 ? (size_t)batch * heads * g.count * key_dim * value_dim * sizeof(float) : 0;
+}
 
 size_t LinearAttention::backward_workspace() const {
-    // f32 partial gradients of every query head, where key/value heads are shared
-    return share() > 1 ? (size_t)tokens() * heads * (key_dim + value_dim) * sizeof(float) : 0;
+    // the segments' states, and f32 partial gradients of every query head where key/value heads are shared
+    return segment_bytes() + (share() > 1 ? (size_t)tokens() * heads * (key_dim + value_dim) * sizeof(float) : 0);
+}
+
+static cudaError_t launch_mix(const MixParams &p, Element e, bool out_f32, void *segments, cudaStream_t s) {
+    if (p.o && chunked_tc_takes(p, e, out_f32)) return launch_chunked_tc(p, out_f32, static_cast<float *>(segments), s);
+    return launch_recurrent(p, e, out_f32, s);
 }
 
 static MixOperand operand(const void *p, const AttentionTensor &t, int per_head) { return {p, t.sb, t.st, t.sh, per_head}; }
@@ -196,6 +205,7 @@ void execute_linear_attention(Context *ctx, const LinearAttention &a, const b200
     check(cudaSetDevice(ctx->device), "cudaSetDevice");
     std::lock_guard<std::mutex> l(ctx->mu);
     if (!stream) stream = ctx->stream;
+    if (!workspace && a.workspace()) workspace = context_scratch(ctx, a.workspace());
     MixParams p = common(ctx, a, b.log_decay, a.packed ? b.sequence_offsets : nullptr);
     p.q = operand(b.query, a.q, 1);
     p.k = operand(b.key, a.k, a.share());
@@ -211,7 +221,7 @@ void execute_linear_attention(Context *ctx, const LinearAttention &a, const b200
     p.dv = (int)a.value_dim;
     p.update = 1.f;
     p.out = a.scale;
-    check(launch_recurrent(p, a.element, false, stream), "kernel launch");
+    check(launch_mix(p, a.element, false, workspace, stream), "kernel launch");
 }
 
 void execute_linear_attention_grad(Context *ctx, const LinearAttention &a,
@@ -252,7 +262,7 @@ void execute_linear_attention_grad(Context *ctx, const LinearAttention &a,
         p.dv = (int)a.key_dim;
         p.update = 1.f;
         p.out = a.scale;
-        check(launch_recurrent(p, a.element, false, stream), "kernel launch");
+        check(launch_mix(p, a.element, false, workspace, stream), "kernel launch");
     }
     // dk and dv run from the last token back; their state is the state's gradient
     auto late = [&](const MixOperand &rq, const MixOperand &rk, const MixOperand &rv, int64_t dk, int64_t dv,
@@ -275,7 +285,7 @@ void execute_linear_attention_grad(Context *ctx, const LinearAttention &a,
             const AttentionTensor dense{a.length * a.heads * dv, a.heads * dv, dv, dv};
             output_to(p, partial, dense);
         }
-        check(launch_recurrent(p, a.element, share > 1, stream), "kernel launch");
+        check(launch_mix(p, a.element, share > 1, workspace, stream), "kernel launch");
         if (share > 1 && out) {
             ShareParams sp{};
             sp.src = partial;
@@ -291,7 +301,7 @@ void execute_linear_attention_grad(Context *ctx, const LinearAttention &a,
             check(launch_share(sp, a.element, stream), "kernel launch");
         }
     };
-    float *part_k = static_cast<float *>(workspace), *part_v = part_k + (share > 1 ? a.tokens() * a.heads * a.key_dim : 0);
+    float *part_k = reinterpret_cast<float *>(static_cast<unsigned char *>(workspace) + a.segment_bytes()), *part_v = part_k + (share > 1 ? a.tokens() * a.heads * a.key_dim : 0);
     // the state's own gradient comes out of the last pass that reads the final state's, which it may replace
     if (g.key_gradient)
         late(v, d, q, a.value_dim, a.key_dim, 1, a.value_dim, g.key_gradient, a.k, part_k,

@@ -67,7 +67,8 @@ struct LinearAttention {
     static LinearAttention from_c(const b200fft_linear_attention_config &c);
     int64_t tokens() const { return packed ? packed_tokens : batch * length; }
     int share() const { return static_cast<int>(heads / kv_heads); }
-    size_t workspace() const;
+    size_t segment_bytes() const;  // states between the segments of the sequences
+    size_t workspace() const { return segment_bytes(); }
     size_t backward_workspace() const;
 };
 
@@ -104,6 +105,17 @@ struct MixParams {
 
 // out_f32: o holds f32 whatever the element type (partial gradients of shared heads)
 cudaError_t launch_recurrent(const MixParams &p, Element e, bool out_f32, cudaStream_t s);
+
+// By chunks of tokens on the tensor cores; segments of a sequence run side by side, with a
+// pass before them that sums up each segment's own state (`segments`: batch x heads x
+// count x dk x dv floats where count > 1).
+struct Segments {
+    int count;   // of the longest sequence
+    int chunks;  // of each segment
+};
+Segments segments_of(int64_t length, int64_t batch, int64_t heads);
+bool chunked_tc_takes(const MixParams &p, Element e, bool out_f32);
+cudaError_t launch_chunked_tc(const MixParams &p, bool out_f32, float *segments, cudaStream_t s);
 
 // dst[.., g, d] = sum over the share query heads of src[token, g * share + j, d]
 struct ShareParams {
