@@ -1,4 +1,4 @@
-// Linear attention by chunks of 128 tokens on the tensor cores (bf16).
+// Linear attention by chunks of 128 tokens on the tensor cores (bf16, f16).
 //
 // With the state S that enters a chunk (rows i, j of the chunk, l the head's decay)
 //   o_i = out * ( sum_{j <= i} l^(i-j) (q_i . k_j) v_j  +  l^(i+1) S^T q_i )
@@ -14,6 +14,10 @@
 //                              bits of the f32 product: the state is an f32 result and stays one
 // The two roundings (P, S) and the result's own are each half a unit of bf16: the result is
 // within sqrt(3) of the rounding that any bf16 result has.
+//
+// f16 has the range of neither scores nor states, so what is rounded to f16 is first multiplied
+// by a power of two, undone in f32: P by row, from the row's largest score; S and W's keys by
+// chunk, from their largest element.  Its two W terms hold 22 bits, f32's own rounding.
 #include <algorithm>
 
 #include "tcgen05.cuh"
@@ -47,7 +51,7 @@ struct Maps {
     CUtensorMap q, k, v, o;
 };
 
-constexpr int kMostShared = 227 * 1024 - 2048;  // of a CTA, beside its static arrays
+constexpr int kMostShared = 227 * 1024;  // of a CTA
 
 template <int DK, int DV>
 struct Layout {
@@ -58,10 +62,34 @@ struct Layout {
     static constexpr int state = 2 * stage;
     static constexpr int turn = state + DK * DV * 2;  // results by stage, where the queries' place is too small
     static constexpr int bytes = turn + (DV > DK ? 2 * (DV / 64) * kPanel : 0);
-    // one CTA per SM: all of tensor memory is its own
-    static constexpr int dynamic = (bytes < 120 * 1024 ? 120 * 1024 : bytes) + 1024;
-    static_assert(dynamic <= kMostShared, "shared memory");
 };
+
+// What a CTA keeps in shared memory beside its tiles.
+struct ChunkSmall {
+    uint64_t bars[16];
+    float column[32], diagonal[32];     // l^n along the columns of a block of scores away from the diagonal, and on it
+                                        // (there times l^-n of the rows or columns, where that stays in range)
+    uint32_t weight[3][kChunk / 2];     // of pairs of tile rows, in terms
+    float pw[kChunk + 4];               // l^n
+    uint32_t tmem_word;
+    int dead, first_odd, odd_values;
+    int careful_at[2];                  // by stage: 0, or which careful chunk it is
+    uint32_t key_most[2][2];            // f16: largest elements of the keys (by stage), of the state, of the rows of
+    uint32_t state_most[2];             // scores (bf16, rounded up)
+    uint16_t row_most[4][kChunk];
+};
+
+// All of the dynamic memory that a kernel asks for: tiles, the rest, and what aligning to 1024 bytes may take.  At
+// least 120 KB: one CTA per SM, as all of tensor memory is its own.
+constexpr int shared_bytes(int tiles, int rest) {
+    const int need = tiles + rest + 1024;
+    return need < 120 * 1024 ? 120 * 1024 : need > kMostShared ? kMostShared : need;
+}
+__device__ __forceinline__ uint32_t dynamic_bytes() {
+    uint32_t n;
+    asm("mov.u32 %0, %%dynamic_smem_size;" : "=r"(n));
+    return n;
+}
 
 template <int DK, int DV>
 struct SumLayout {
@@ -70,8 +98,6 @@ struct SumLayout {
     static constexpr int stage = v + (DV / 64) * kPanel;
     static constexpr int stages = 3;
     static constexpr int bytes = stages * stage;
-    static constexpr int dynamic = (bytes < 120 * 1024 ? 120 * 1024 : bytes) + 1024;
-    static_assert(dynamic <= kMostShared, "shared memory");
 };
 
 // l s as s + (l - 1) s where l is near one, so that many chunks do not add up l's rounding.
@@ -88,17 +114,55 @@ __device__ __forceinline__ uint32_t tile_byte(int r, int c, int rows) {
     return (c >> 6) * (rows * 128) + r * 128 + ((((c >> 3) & 7) ^ (r & 7)) << 4) + (c & 7) * 2;
 }
 
+template <typename T>
 __device__ __forceinline__ float tile_value(const unsigned char *t, int r, int c, int rows) {
-    return __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(t + tile_byte(r, c, rows)));
+    return to_float(*reinterpret_cast<const T *>(t + tile_byte(r, c, rows)));
 }
 
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&v);
+// Two elements in a register.
+template <typename T>
+struct Two;
+template <>
+struct Two<__nv_bfloat16> {
+    using type = __nv_bfloat162;
+    static constexpr uint32_t exponent = 0x7f807f80u, above = 0x00800080u;  // exponent + above: a sign where it is all ones
+    static __device__ __forceinline__ type of(float a, float b) { return __floats2bfloat162_rn(a, b); }
+    static __device__ __forceinline__ float2 wide(type v) { return __bfloat1622float2(v); }
+};
+template <>
+struct Two<__half> {
+    using type = __half2;
+    static constexpr uint32_t exponent = 0x7c007c00u, above = 0x04000400u;
+    static __device__ __forceinline__ type of(float a, float b) { return __floats2half2_rn(a, b); }
+    static __device__ __forceinline__ float2 wide(type v) { return __half22float2(v); }
+};
+template <typename T>
+__device__ __forceinline__ typename Two<T>::type as_two(uint32_t v) { return *reinterpret_cast<const typename Two<T>::type *>(&v); }
+template <typename P>
+__device__ __forceinline__ uint32_t as_word(P v) { return *reinterpret_cast<const uint32_t *>(&v); }
+template <typename T>
+__device__ __forceinline__ uint32_t pack(float a, float b) { return as_word(Two<T>::of(a, b)); }
+// Two f32 as the sums of three (two) terms each.
+template <typename T, int TERMS>
+__device__ __forceinline__ void split_terms(float a, float b, uint32_t *t, int step) {
+#pragma unroll
+    for (int k = 0; k < TERMS; k++) {
+        t[k * step] = pack<T>(a, b);
+        const float2 w = Two<T>::wide(as_two<T>(t[k * step]));
+        a -= w.x;
+        b -= w.y;
+    }
 }
 
-__device__ __forceinline__ __nv_bfloat162 as_pair(uint32_t v) { return *reinterpret_cast<const __nv_bfloat162 *>(&v); }
-__device__ __forceinline__ uint32_t as_word(__nv_bfloat162 v) { return *reinterpret_cast<const uint32_t *>(&v); }
+// The power of two that brings `most` to [2^top, 2^(top+1)), held within 2^-60 and 2^60, and its inverse.
+// `most` is not negative; where it is no number, or infinite, anything goes.
+struct Scale {
+    float up, down;
+};
+__device__ __forceinline__ Scale scale_to(float most, int top) {
+    const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, top - 60), top + 60);
+    return {__uint_as_float((uint32_t)(127 + top - e) << 23), __uint_as_float((uint32_t)(127 - top + e) << 23)};
+}
 
 // Barrier 1: the compute warps among themselves.
 __device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kComputeWarps * 32) : "memory"); }
@@ -136,7 +200,7 @@ __device__ __forceinline__ float *segment_state(const ChunkParams &cp, int64_t b
 // The rows of a chunk from the first on whose value holds an infinity or NaN, one by one: the
 // tensor cores' product with a masked score of zero would spread it to tokens before it, so
 // those get the product again without it, and the rest comes from here.  Rare and slow.
-template <int DK, int DV>
+template <typename T, int DK, int DV>
 __device__ __noinline__ void careful_rows(const unsigned char *sq, const unsigned char *sk, const unsigned char *sv,
                                           const unsigned char *ss, const float *pw, int first, int last, int from, int reverse,
                                           float inside, float before, void *out, int64_t ost, int dv, int out_f32) {
@@ -147,19 +211,19 @@ __device__ __noinline__ void careful_rows(const unsigned char *sq, const unsigne
 #pragma unroll
         for (int m = 0; m < DV / 32; m++) acc[m] = state[m] = 0.f;
         for (int d = 0; d < DK; d++) {
-            const float q = tile_value(sq, i, d, kChunk);
+            const float q = tile_value<T>(sq, i, d, kChunk);
 #pragma unroll
-            for (int m = 0; m < DV / 32; m++) state[m] = fmaf(q, tile_value(ss, d, lane + 32 * m, DK), state[m]);
+            for (int m = 0; m < DV / 32; m++) state[m] = fmaf(q, tile_value<T>(ss, d, lane + 32 * m, DK), state[m]);
         }
         const int j0 = reverse ? i : first, j1 = reverse ? last : i + 1;
         for (int j = j0; j < j1; j++) {
             float dot = 0.f;
 #pragma unroll
             for (int m = 0; m < DK / 32; m++)
-                dot = fmaf(tile_value(sq, i, lane + 32 * m, kChunk), tile_value(sk, j, lane + 32 * m, kChunk), dot);
+                dot = fmaf(tile_value<T>(sq, i, lane + 32 * m, kChunk), tile_value<T>(sk, j, lane + 32 * m, kChunk), dot);
             const float score = warp_sum(dot) * (inside * pw[reverse ? j - i : i - j]);
 #pragma unroll
-            for (int m = 0; m < DV / 32; m++) acc[m] = fmaf(score, tile_value(sv, j, lane + 32 * m, kChunk), acc[m]);
+            for (int m = 0; m < DV / 32; m++) acc[m] = fmaf(score, tile_value<T>(sv, j, lane + 32 * m, kChunk), acc[m]);
         }
         const float fade = before * pw[reverse ? kChunk - 1 - i : i + 1];
 #pragma unroll
@@ -170,35 +234,40 @@ __device__ __noinline__ void careful_rows(const unsigned char *sq, const unsigne
             if (out_f32)
                 static_cast<float *>(out)[i * ost + c] = v;
             else
-                static_cast<__nv_bfloat16 *>(out)[i * ost + c] = __float2bfloat16_rn(v);
+                static_cast<T *>(out)[i * ost + c] = from_float<T>(v);
         }
     }
 }
 
-// W of 16 tile rows and 32 key columns: the weights w = w1 + w2 + w3 (bf16 terms) of this thread's rows, 2 (lane % 4),
-// 2 (lane % 4) + 1 and those 8 further on, times the keys.  k w1 = a + b and k w2 = c + d exactly (a product of two
-// 8-bit mantissas is its rounding and a bf16 remainder), so W = a + b + c + (d + k w3): only the last sum is rounded,
-// at 2^-25 of W.  Two terms are a and b + k w2, off by 2^-17.  Packed bf16 arithmetic: five (three) instructions for
-// two rows; terms cut out of the f32 product took twice as many.  ldmatrix turns the keys the way the tensor memory
-// wants them (a lane for each key column): one 2-byte load for each key had bound this step.
-template <int TERMS>
-__device__ __forceinline__ void make_weights(uint32_t keys, uint32_t unit, const uint32_t (&w)[3][2], uint32_t to, int term_columns) {
+// W of 16 tile rows and 32 key columns: the weights w = w1 + w2 + w3 (terms of the type) of this thread's rows,
+// 2 (lane % 4), 2 (lane % 4) + 1 and those 8 further on, times the keys.  k w1 = a + b and k w2 = c + d exactly (a
+// product of two mantissas is its rounding and a remainder of the type), so W = a + b + c + (d + k w3): only the last
+// sum is rounded, at 2^-25 of W in bf16.  Two terms are a and b + k w2, off by 2^-17 (f16: 2^-23).  Packed 16-bit
+// arithmetic: five (three) instructions for two rows; terms cut out of the f32 product took twice as many.  ldmatrix
+// turns the keys the way the tensor memory wants them (a lane for each key column): one 2-byte load for each key had
+// bound this step.
+template <typename T, int TERMS>
+__device__ __forceinline__ void make_weights(uint32_t keys, uint32_t unit, uint32_t key_scale, const uint32_t (&w)[3][2],
+                                             uint32_t to, int term_columns) {
+    using P = typename Two<T>::type;
 #pragma unroll
     for (int half = 0; half < 2; half++) {  // 16 key columns
         uint32_t k4[4], t[TERMS][4];
         load_blocks_transposed(keys + (unit ^ (half << 5)), k4);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const __nv_bfloat162 k = as_pair(k4[e]), w1 = as_pair(w[0][e >> 1]), w2 = as_pair(w[1][e >> 1]);
-            const __nv_bfloat162 a = __hmul2_rn(k, w1), b = __hfma2(k, w1, __hneg2(a));
+            P k = as_two<T>(k4[e]);
+            if (std::is_same<T, __half>::value) k = __hmul2_rn(k, as_two<T>(key_scale));
+            const P w1 = as_two<T>(w[0][e >> 1]), w2 = as_two<T>(w[1][e >> 1]);
+            const P a = __hmul2_rn(k, w1), b = __hfma2(k, w1, __hneg2(a));
             t[0][e] = as_word(a);
             if (TERMS == 2) {
                 t[1][e] = as_word(__hfma2(k, w2, b));
             } else {
-                const __nv_bfloat162 c = __hmul2_rn(k, w2), d = __hfma2(k, w2, __hneg2(c));
+                const P c = __hmul2_rn(k, w2), d = __hfma2(k, w2, __hneg2(c));
                 t[1][e] = as_word(b);
                 t[2][e] = as_word(c);
-                t[3][e] = as_word(__hfma2(k, as_pair(w[2][e >> 1]), d));
+                t[3][e] = as_word(__hfma2(k, as_two<T>(w[2][e >> 1]), d));
             }
         }
 #pragma unroll
@@ -207,7 +276,38 @@ __device__ __forceinline__ void make_weights(uint32_t keys, uint32_t unit, const
     }
 }
 
-// Loads the tiles that zeroing rows outside the sequence leaves: keys and values stand behind one another.
+// f16: the keys' largest finite element decides the power of two that they are multiplied by (at most 2^15), and the
+// weights come at 2^14: no term of W overflows, and what falls below f16's range is below 2^-30 of the largest.
+constexpr int kWeightBits = 14;
+__device__ __forceinline__ Scale key_scale_of(uint32_t most) {  // f16 bits
+    const float m = __half2float(__ushort_as_half((unsigned short)most));
+    Scale k = scale_to(fmaxf(m, 1.f / 32768.f), 0);
+    k.down *= 1.f / (1 << kWeightBits);  // undoes the weights' factor too
+    return k;
+}
+__device__ __forceinline__ uint32_t finite_max2(uint32_t most, uint32_t word) {  // by halves, of absolute f16 values
+    const uint32_t a = word & 0x7fff7fffu;
+    return __vmaxu2(most, a & ~(__vcmpgeu2(a, 0x7c007c00u)));
+}
+
+// One of two warps: the largest finite absolute value (f16 bits) in its half of the valid rows.
+template <int DK>
+__device__ __forceinline__ uint32_t largest_key(const unsigned char *keys, int which, int first, int end) {
+    const int lane = threadIdx.x & 31;
+    uint32_t most = 0;
+    for (int panel = 0; panel < DK / 64; panel++)
+#pragma unroll 4
+        for (int u = 0; u < 16; u++) {  // four rows at a time
+            const uint4 w = *reinterpret_cast<const uint4 *>(keys + panel * kPanel + which * 64 * 128 + u * 512 + lane * 16);
+            const int r = which * 64 + u * 4 + (lane >> 3);
+            uint32_t here = finite_max2(finite_max2(0, w.x), w.y);
+            here = finite_max2(finite_max2(here, w.z), w.w);
+            if (r >= first && r < end) most = __vmaxu2(most, here);
+        }
+    return __reduce_max_sync(~0u, max(most & 0xffff, most >> 16));
+}
+
+// Zeroes the rows outside the sequence, of keys and of the values behind them.
 template <int BYTES>
 __device__ __forceinline__ void clear_rows(unsigned char *tiles, int first, int end) {
     for (int u = threadIdx.x; u < BYTES / 16; u += kComputeWarps * 32) {
@@ -219,19 +319,26 @@ __device__ __forceinline__ void clear_rows(unsigned char *tiles, int first, int 
 }
 
 // A segment's own sum: what its tokens leave of the state at its end, from a state of zero.  The weights reach to the
-// end of the segment, so that all chunks add up in tensor memory; four terms, as it is an f32 result.
-template <int DK, int DV>
+// end of the segment, so that all chunks add up in tensor memory; four terms, as it is an f32 result.  f16, whose keys
+// are scaled by chunk, adds the chunks up in registers instead, one chunk behind the products.
+template <typename T, int DK, int DV>
 __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant__ Maps maps,
                                                           const __grid_constant__ ChunkParams cp) {
     using L = SumLayout<DK, DV>;
     constexpr int COLS = DV / kGroups;
+    constexpr bool HALF = std::is_same<T, __half>::value;
+    constexpr int TERMS = HALF ? 2 : 4;
     constexpr int kBuffers = 3;                         // of W for half a chunk
-    constexpr uint32_t buffer_column[kBuffers] = {0, 128, 384};
+    // columns: W buffers; the sum of all chunks, or of two chunks in turn
+    constexpr uint32_t kW0 = 0, kW1 = HALF ? 64 : 128, kW2 = HALF ? 128 : 384;
+    constexpr uint32_t kSums = 256;
     extern __shared__ unsigned char raw[];
-    __shared__ __align__(8) uint64_t bars[2 * L::stages + 2 * kBuffers + 1];
+    __shared__ __align__(8) uint64_t bars[3 * L::stages + 2 * kBuffers + 2];
     __shared__ uint32_t tmem_word;
     __shared__ int dead;
-    __shared__ float pw[kChunk + 1];  // update * l^n
+    __shared__ float pw[kChunk + 1];  // l^n, times `update` or f16's weight factor
+    __shared__ uint32_t key_most[2][L::stages];
+    auto buffer_at = [](int i) { return i == 0 ? kW0 : i == 1 ? kW1 : kW2; };
 
     const MixParams &p = cp.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -245,16 +352,18 @@ __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant_
     const uint32_t base = shared_address(smem), bar0 = shared_address(bars);
     const uint32_t full = bar0, free = bar0 + 8 * L::stages;                       // tiles have come; are used up
     const uint32_t ready = bar0 + 16 * L::stages, used = ready + 8 * kBuffers;     // W is in place; is used up
-    const uint32_t all = used + 8 * kBuffers;
+    const uint32_t sums = used + 8 * kBuffers;                                     // a chunk's, or all chunks', products
+    const uint32_t scanned = sums + 16;                                            // (f16) the keys' largest is known
     if (warp == 0) tmem_alloc(shared_address(&tmem_word), kTmemColumns);
     if (tid == 0) {
-        for (int k = 0; k < 2 * L::stages + 2 * kBuffers + 1; k++)
+        for (int k = 0; k < 2 * L::stages + 2 * kBuffers + 2; k++)
             barrier_init(bar0 + 8 * k, k >= 2 * L::stages && k < 2 * L::stages + kBuffers ? kComputeWarps : 1);
+        for (int k = 0; k < L::stages; k++) barrier_init(scanned + 8 * k, 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         dead = 0;
     }
     const float log_decay = p.log_decay[h];
-    if (tid <= kChunk) pw[tid] = (float)((tid ? exp((double)log_decay * tid) : 1.0) * p.update);
+    if (tid <= kChunk) pw[tid] = (float)((tid ? exp((double)log_decay * tid) : 1.0) * (HALF ? 1 << kWeightBits : p.update));
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
@@ -267,13 +376,38 @@ __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant_
         const uint32_t lanes = tmem + ((uint32_t)(block * 32) << 16);
         const uint32_t keys = base + L::k + (block >> 1) * kPanel + ((lane & 7) + (lane >> 4) * 8) * 128;
         const uint32_t unit = (((block & 1) * 4 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4;
+        float s[COLS];
+#pragma unroll
+        for (int j = 0; j < COLS; j++) s[j] = 0.f;
+        Scale before{1.f, 1.f};
+        const Fade whole = fade_of((double)log_decay * kChunk);
+        // reverse: the decay of a row itself; f16 multiplies by it here, as its weights would underflow together
+        constexpr int OWN = HALF ? 0 : 1;
+        const float factor = p.update * (p.reverse ? expf(log_decay) : 1.f);
+        auto add = [&](int c, int n, float down) {  // f16: s <- l^n s + the products of chunk c
+            barrier_wait(sums + 8 * (c & 1), (c >> 1) & 1, gone);
+            fence_after_sync();
+            if (row >= DK) return;
+            const Fade keep = n == kChunk ? whole : fade_of((double)log_decay * n);
+            uint32_t x[COLS];
+            tmem_load(lanes + kSums + (c & 1) * 128 + group * COLS, x);
+#pragma unroll
+            for (int j = 0; j < COLS; j++) s[j] = fmaf(__uint_as_float(x[j]), down * factor, faded(s[j], keep));
+        };
         for (int c = 0; c < chunks; c++) {
             const int stage = c % L::stages, n = min(kChunk, line.tokens - c * kChunk);
             const int first = p.reverse ? kChunk - n : 0, end = first + n;
             // l^(tokens of the segment after this chunk)
-            const float later = expf(log_decay * (float)max(line.tokens - (c + 1) * kChunk, 0));
+            const int after = HALF ? 0 : max(line.tokens - (c + 1) * kChunk, 0);
+            const float later = expf(log_decay * (float)after);
             barrier_wait(full + 8 * stage, (c / L::stages) & 1, gone);
             if (n < kChunk) clear_rows<L::stage>(smem + stage * L::stage, first, end);
+            Scale key{1.f, 1.f};
+            if (HALF) {
+                barrier_wait(scanned + 8 * stage, (c / L::stages) & 1, gone);
+                key = key_scale_of(max(key_most[0][stage], key_most[1][stage]));
+            }
+            const uint32_t key_factor = HALF ? pack<T>(key.up, key.up) : 0;
 #pragma unroll
             for (int half = 0; half < 2; half++) {
                 const int i = 2 * c + half, buffer = i % kBuffers, r0 = half * 64 + group * 16 + 2 * (lane & 3);
@@ -284,35 +418,39 @@ __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant_
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const int r = r0 + 8 * pair + e;
-                        f[e] = r >= first && r < end ? pw[p.reverse ? r + 1 - first : end - 1 - r] : 0.f;
-                        if (line.tokens - (c + 1) * kChunk > 0) f[e] *= later;
+                        f[e] = r >= first && r < end ? pw[p.reverse ? r + OWN - first : end - 1 - r] : 0.f;
+                        if (after > 0) f[e] *= later;
                     }
-#pragma unroll
-                    for (int term = 0; term < 3; term++) {
-                        const uint32_t t = pack_bf16(f[0], f[1]);
-                        w[term][pair] = t;
-                        f[0] -= __uint_as_float(t << 16);
-                        f[1] -= __uint_as_float(t & 0xffff0000u);
-                    }
+                    split_terms<T, TERMS == 2 ? 2 : 3>(f[0], f[1], &w[0][pair], 2);
                 }
                 if (i >= kBuffers) {
                     barrier_wait(used + 8 * buffer, (i / kBuffers - 1) & 1, gone);
                     fence_after_sync();
                 }
                 if (row < DK)
-                    make_weights<4>(keys + stage * L::stage + (half * 4 + group) * 2048, unit, w,
-                                    lanes + buffer_column[buffer] + group * 8, 32);
+                    make_weights<T, TERMS>(keys + stage * L::stage + (half * 4 + group) * 2048, unit, key_factor, w,
+                                    lanes + buffer_at(buffer) + group * 8, 32);
                 tmem_store_wait();
                 fence_before_sync();
                 __syncwarp();
                 if (lane == 0) barrier_arrive(ready + 8 * buffer);
             }
+            if (HALF) {
+                if (c > 0) add(c - 1, kChunk, before.down);
+                before = key;
+            }
         }
-        barrier_wait(all, 0, gone);
+        if (HALF) add(chunks - 1, line.tokens - (chunks - 1) * kChunk, before.down);
+        if (!HALF) barrier_wait(sums, 0, gone);
         fence_after_sync();
         if (row < DK) {
             uint32_t x[COLS];
-            tmem_load(lanes + kZ + group * COLS, x);
+            if (HALF) {
+#pragma unroll
+                for (int j = 0; j < COLS; j++) x[j] = __float_as_uint(s[j]);
+            } else {
+                tmem_load(lanes + kSums + group * COLS, x);
+            }
             if (row < p.dk) {
                 float *to = segment_state(cp, b, h, segment) + row * p.dv;
 #pragma unroll
@@ -331,17 +469,18 @@ __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant_
                     const uint64_t v = values + ((base + stage * L::stage + L::v + (i & 1) * 64 * 128) >> 4);
                     barrier_wait(ready + 8 * buffer, (i / kBuffers) & 1, gone);
                     fence_after_sync();
-                    const uint32_t w = tmem + buffer_column[buffer];
+                    const uint32_t w = tmem + buffer_at(buffer);
 #pragma unroll
-                    for (int term = 0; term < 4; term++)
+                    for (int term = 0; term < TERMS; term++)
 #pragma unroll
                         for (int n = 0; n < 4; n++)
-                            mma_tensor(tmem + kZ, w + term * 32 + n * 8, v + (n * 2048 >> 4), mma_desc(DV, true),
-                                       i > 0 || term > 0 || n > 0);
+                            mma_tensor(tmem + kSums + (HALF ? (i >> 1 & 1) * 128 : 0), w + term * 32 + n * 8, v + (n * 2048 >> 4),
+                                       mma_desc<T>(DV, true), (HALF ? i & 1 : i) > 0 || term > 0 || n > 0);
                     mma_commit(used + 8 * buffer);
                     if (i & 1) mma_commit(free + 8 * stage);
+                    if (HALF && (i & 1)) mma_commit(sums + 8 * (i >> 1 & 1));
                 }
-                mma_commit(all);
+                if (!HALF) mma_commit(sums);
             }
         } else if (warp == kComputeWarps + 1) {
             if (lane == 0) {
@@ -363,6 +502,19 @@ __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant_
                     for (int i = 0; i < 1 << 18 && !barrier_try(full + 8 * (e % L::stages), (e / L::stages) & 1); i++) {
                     }
             }
+        } else if (HALF) {
+            const int which = warp - kComputeWarps - 2;
+            for (int c = 0; c < chunks; c++) {
+                const int stage = c % L::stages, n = min(kChunk, line.tokens - c * kChunk);
+                const int first = p.reverse ? kChunk - n : 0;
+                barrier_wait(full + 8 * stage, (c / L::stages) & 1, gone);
+                const uint32_t most = largest_key<DK>(smem + stage * L::stage + L::k, which, first, first + n);
+                if (lane == 0) {
+                    key_most[which][stage] = most;
+                    barrier_arrive(scanned + 8 * stage);
+                }
+                __syncwarp();
+            }
         }
     }
     fence_before_sync();
@@ -371,26 +523,17 @@ __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant_
     if (warp == 0) tmem_free(tmem, kTmemColumns);
 }
 
-// The results of a segment, and (one segment) the final state.
-// TERMS: bf16 terms of the state update's weights.  Two (2^-17) where the state only goes on into results; four where
-// it is itself a result, in f32: then the weights of half a chunk fill the tensor memory that is left.
-template <int DK, int DV, int TERMS>
+// The results of a segment, and (FINAL, one segment) the final state.
+// bf16 terms of the state update's weights: two (2^-17) where the state only goes on into results; four where it is
+// itself a result, in f32: then the weights of half a chunk fill the tensor memory that is left.
+template <typename T, int DK, int DV, bool FINAL>
 __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constant__ Maps maps,
                                                             const __grid_constant__ ChunkParams cp) {
     using L = Layout<DK, DV>;
     constexpr int COLS = DV / kGroups;  // state and result columns of one thread
-    constexpr int HALVES = TERMS == 4 ? 2 : 1, kTermColumns = kChunk / 2 / HALVES;
+    constexpr bool HALF = std::is_same<T, __half>::value;
+    constexpr int TERMS = FINAL && !HALF ? 4 : 2, HALVES = TERMS == 4 ? 2 : 1, kTermColumns = kChunk / 2 / HALVES;
     extern __shared__ unsigned char raw[];
-    __shared__ __align__(8) uint64_t bars[14];
-    __shared__ uint32_t tmem_word;
-    __shared__ int dead, first_odd, odd_values;
-    __shared__ int careful_at[2];                              // by stage: 0, or which careful chunk it is
-    __shared__ float pw[kChunk + 1];                           // l^n
-    __shared__ __align__(16) uint32_t weight[3][kChunk / 2];   // of pairs of tile rows, as three bf16 terms
-    // l^n along the columns of a block of scores away from the diagonal, and on it (there times l^-n of the
-    // rows or columns, where that stays in range)
-    __shared__ __align__(16) float column[32], diagonal[32];
-
     const MixParams &p = cp.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int segment = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
@@ -408,6 +551,20 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
 
     unsigned char *smem = raw + ((1024 - (shared_address(raw) & 1023)) & 1023);
     const uint32_t base = shared_address(smem);
+    if (base + L::bytes + sizeof(ChunkSmall) > shared_address(raw) + dynamic_bytes()) {  // no room after aligning
+        if (tid == 0) atomicOr(p.err, 64);
+        return;
+    }
+    ChunkSmall &small = *reinterpret_cast<ChunkSmall *>(smem + L::bytes);
+    auto &bars = small.bars;
+    auto &weight = small.weight;
+    auto &careful_at = small.careful_at;
+    auto &key_most = small.key_most;
+    auto &state_most = small.state_most;
+    auto &row_most = small.row_most;
+    float *const pw = small.pw, *const column = small.column, *const diagonal = small.diagonal;
+    int &dead = small.dead, &first_odd = small.first_odd, &odd_values = small.odd_values;
+    uint32_t &tmem_word = small.tmem_word;
     const uint32_t bar0 = shared_address(bars);
     // by stage: tiles have come; every compute warp is done with a chunk
     const uint32_t full = bar0, done = bar0 + 16;
@@ -416,13 +573,15 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                    bar_again = bar0 + 72;
     // operands that every warp concerned has put in place
     const uint32_t w0_ready = bar0 + 80, w1_ready = bar0 + 88, p_ready = bar0 + 96, v_ready = bar0 + 104;
+    const uint32_t scanned = bar0 + 112;  // by stage (f16): the keys' largest is known
     if (warp == 0) tmem_alloc(shared_address(&tmem_word), kTmemColumns);
     if (tid == 0) {
-        for (int k = 0; k < 14; k++)
-            barrier_init(bar0 + 8 * k, k == 12 ? kComputeWarps + 2 : k == 2 || k == 3 || k >= 10 ? kComputeWarps : 1);
+        for (int k = 0; k < 16; k++)
+            barrier_init(bar0 + 8 * k, k >= 14 ? 2 : k == 12 ? kComputeWarps + 2 : k == 2 || k == 3 || k >= 10 ? kComputeWarps : 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         dead = odd_values = 0;
         careful_at[0] = careful_at[1] = 0;
+        state_most[0] = state_most[1] = 0;
     }
     const float log_decay = p.log_decay[h];
     if (tid <= kChunk) {
@@ -456,15 +615,32 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
 
         // the state: row `row`, columns from group * COLS
         float s[COLS];
-        auto publish_state = [&] {
+        Scale state{1.f, 1.f}, key{1.f, 1.f};
+        auto publish_state = [&](int which) {
+            if (HALF) {  // the scale is everyone's
+                float most = 0.f;
+#pragma unroll
+                for (int c = 0; c < COLS; c++) most = fmaxf(most, fabsf(s[c]));
+                const uint32_t bits = __reduce_max_sync(~0u, most <= 3.4e38f ? __float_as_uint(most) : 0u);
+                if (lane == 0) atomicMax(&state_most[which], bits);
+                compute_sync();
+                state = scale_to(__uint_as_float(*(volatile uint32_t *)&state_most[which]), 14);
+                if (tid == 0) state_most[which ^ 1] = 0;  // used again after every warp has been waited for
+#pragma unroll
+                for (int c = 0; c < COLS; c++) s[c] *= state.up;
+            }
             if (state_row) {
 #pragma unroll
                 for (int c = 0; c < COLS; c += 8) {
                     uint4 v;
-                    v.x = pack_bf16(s[c], s[c + 1]), v.y = pack_bf16(s[c + 2], s[c + 3]);
-                    v.z = pack_bf16(s[c + 4], s[c + 5]), v.w = pack_bf16(s[c + 6], s[c + 7]);
+                    v.x = pack<T>(s[c], s[c + 1]), v.y = pack<T>(s[c + 2], s[c + 3]);
+                    v.z = pack<T>(s[c + 4], s[c + 5]), v.w = pack<T>(s[c + 6], s[c + 7]);
                     *reinterpret_cast<uint4 *>(state_tile + tile_byte(row, group * COLS + c, DK)) = v;
                 }
+            }
+            if (HALF) {
+#pragma unroll
+                for (int c = 0; c < COLS; c++) s[c] *= state.down;  // a power of two: exact
             }
             fence_async_shared();
         };
@@ -485,7 +661,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                         s[c + e] = in && row < p.dk && col + e < p.dv ? in[row * in_k + (col + e) * in_v] : 0.f;
                 }
             }
-            publish_state();
+            publish_state(1);
             arrive(done + 8);
         }
 
@@ -494,6 +670,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         // blocks of keys as ldmatrix reads them: lane i names row i % 8 + 8 (i / 16) and 8 columns, i / 8 % 2
         const uint32_t keys = base + L::k + (block >> 1) * kPanel + ((lane & 7) + (lane >> 4) * 8) * 128;
         const uint32_t unit = (((block & 1) * 4 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4;
+        // reverse: the decay of a row itself; f16 multiplies by it in f32, as its weights would underflow together
+        constexpr int OWN = HALF ? 0 : 1;
         const bool gentle = log_decay > -2.5f;  // l^-31 is in range
         for (int c = 0; c < chunks; c++) {
             const int parity = c & 1;
@@ -510,21 +688,22 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const int r = 2 * tid + e;
-                        w[e] = r >= first && r < end ? p.update * pw[p.reverse ? r + 1 - first : end - 1 - r] : 0.f;
+                        w[e] = r >= first && r < end ? (HALF ? (float)(1 << kWeightBits) : p.update) *
+                                                           pw[p.reverse ? r + OWN - first : end - 1 - r] : 0.f;
                     }
-#pragma unroll
-                    for (int term = 0; term < 3; term++) {
-                        const uint32_t t = pack_bf16(w[0], w[1]);
-                        weight[term][tid] = t;
-                        w[0] -= __uint_as_float(t << 16);
-                        w[1] -= __uint_as_float(t & 0xffff0000u);
-                    }
+                    split_terms<T, 3>(w[0], w[1], &weight[0][tid], kChunk / 2);
                 }
                 compute_sync();
             }
             barrier_wait(full + 8 * (c & 1), (c >> 1) & 1, gone);
             if (n < kChunk) clear_rows<L::stage - L::k>(tile + L::k, first, end);
 
+            uint32_t key_factor = 0;
+            if (HALF) {
+                barrier_wait(scanned + 8 * (c & 1), (c >> 1) & 1, gone);
+                key = key_scale_of(max(key_most[0][c & 1], key_most[1][c & 1]));
+                key_factor = pack<T>(key.up, key.up);
+            }
             // W of 16 rows
             auto weigh = [&](int at, int column) {
                 if (!state_row) return;
@@ -534,7 +713,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                     w[term][0] = weight[term][at * 8 + (lane & 3)];
                     w[term][1] = weight[term][at * 8 + (lane & 3) + 4];
                 }
-                make_weights<TERMS>(keys + (c & 1) * L::stage + at * 2048, unit, w, lanes + kW + column, kTermColumns);
+                make_weights<T, TERMS>(keys + (c & 1) * L::stage + at * 2048, unit, key_factor, w, lanes + kW + column, kTermColumns);
             };
             if (HALVES == 2) {
                 weigh(group, group * 8);
@@ -545,27 +724,30 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
             tmem_store_wait();
             arrive(w0_ready);
 
-            // scores -> P in place: a block of 32 columns leaves 16 columns of bf16 pairs behind
+            // scores -> P in place: a block of 32 columns leaves 16 columns of pairs behind
             barrier_wait(bar_x, parity, gone);
             fence_after_sync();
+            Scale scores{1.f, 1.f};  // f16: of this row
             {
                 const uint32_t at = lanes + kX + group * 32;
                 uint32_t packed[16];
-                if (p.reverse ? group < block : group > block) {  // all of it lies ahead
+                const bool on = group == block, none = p.reverse ? group < block : group > block;  // all of it lies ahead
+                uint32_t x[32];
+                if (none) {
 #pragma unroll
                     for (int j = 0; j < 16; j++) packed[j] = 0;
                 } else {
-                    uint32_t x[32];
                     tmem_load(at, x);
-                    const bool on = group == block;
                     if (on && !gentle) {
 #pragma unroll
                         for (int j = 0; j < 32; j++) {
                             const int gap = p.reverse ? j - lane : lane - j;
                             x[j] = gap >= 0 ? __float_as_uint(__uint_as_float(x[j]) * (inside * pw[max(gap, 0)])) : 0;
                         }
+                        if (!HALF) {
 #pragma unroll
-                        for (int j = 0; j < 16; j++) packed[j] = pack_bf16(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]));
+                            for (int j = 0; j < 16; j++) packed[j] = pack<T>(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]));
+                        }
                     } else {
                         const float f = inside * (on ? (p.reverse ? 1.f / pw[lane] : pw[lane])
                                                      : pw[p.reverse ? group * 32 - row : row - group * 32 - 31]);
@@ -579,10 +761,15 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                                                 mul_pair(ff, pair_of(w.x, w.y))), y[0], y[1]);
                             split_pair(mul_pair(pair_of(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])),
                                                 mul_pair(ff, pair_of(w.z, w.w))), y[2], y[3]);
-                            packed[j / 2] = pack_bf16(y[0], y[1]);
-                            packed[j / 2 + 1] = pack_bf16(y[2], y[3]);
+                            if (HALF) {
+#pragma unroll
+                                for (int e = 0; e < 4; e++) x[j + e] = __float_as_uint(y[e]);
+                            } else {
+                                packed[j / 2] = pack<T>(y[0], y[1]);
+                                packed[j / 2 + 1] = pack<T>(y[2], y[3]);
+                            }
                         }
-                        if (on) {  // columns ahead of this row: a shift by 0, 16 or 32 bits leaves none, one or both
+                        if (!HALF && on) {  // columns ahead of this row: a shift by 0, 16 or 32 bits leaves none, one or both
                             if (p.reverse) {
 #pragma unroll
                                 for (int j = 0; j < 16; j++) packed[j] &= __funnelshift_rc(0, ~0u, max(32 * j + 32 - 16 * lane, 0));
@@ -593,13 +780,32 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                         }
                     }
                 }
+                if (HALF) {
+                    float most = 0.f;
+                    if (!none) {
+#pragma unroll
+                        for (int j = 0; j < 32; j++) {
+                            if (on) x[j] = (p.reverse ? j >= lane : j <= lane) ? x[j] : 0;
+                            most = fmaxf(most, fabsf(__uint_as_float(x[j])));
+                        }
+                    }
+                    row_most[group][row] = (uint16_t)((__float_as_uint(most) >> 16) + 1);  // its upper half, no less
+                    asm volatile("bar.sync %0, 128;" ::"r"(3 + block) : "memory");  // the warps that share these rows
+                    scores = scale_to(__uint_as_float((uint32_t)max(max(row_most[0][row], row_most[1][row]),
+                                                                    max(row_most[2][row], row_most[3][row])) << 16), 14);
+                    if (!none) {
+#pragma unroll
+                        for (int j = 0; j < 16; j++)
+                            packed[j] = pack<T>(__uint_as_float(x[2 * j]) * scores.up, __uint_as_float(x[2 * j + 1]) * scores.up);
+                    }
+                }
                 tmem_store(at, packed);
             }
             // the state's part of the result, faded by row; the product inside the chunk adds to it
             barrier_wait(bar_y, parity, gone);
             fence_after_sync();
             {
-                const float fade = p.out * pw[p.reverse ? kChunk - 1 - row : row + 1];
+                const float fade = p.out * pw[p.reverse ? kChunk - 1 - row : row + 1] * (HALF ? state.down : 1.f) * scores.up;
                 uint32_t x[COLS];
                 tmem_load(lanes + kY + group * COLS, x);
 #pragma unroll
@@ -628,11 +834,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                     uint32_t x[COLS];
                     tmem_load(lanes + kZ + group * COLS, x);
                     const uint64_t whole = pair_of(keep.whole, keep.whole), rest = pair_of(keep.rest, keep.rest);
+                    const float factor = key.down * p.update * (p.reverse ? pw[1] : 1.f);
+                    const uint64_t down = pair_of(factor, factor);
 #pragma unroll
                     for (int j = 0; j < COLS; j += 2) {
                         const uint64_t old = pair_of(s[j], s[j + 1]);
-                        split_pair(add_pair(fma_pair(old, rest, mul_pair(old, whole)),
-                                            pair_of(__uint_as_float(x[j]), __uint_as_float(x[j + 1]))), s[j], s[j + 1]);
+                        const uint64_t more = pair_of(__uint_as_float(x[j]), __uint_as_float(x[j + 1]));
+                        const uint64_t kept = fma_pair(old, rest, mul_pair(old, whole));
+                        split_pair(HALF ? fma_pair(more, down, kept) : add_pair(more, kept), s[j], s[j + 1]);
                     }
                 }
             };
@@ -655,20 +864,20 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                     compute_sync();
                     for (int u = tid; u < kChunk * DV; u += kComputeWarps * 32) {
                         const int r = u / DV;
-                        const float v = tile_value(sv, r, u % DV, kChunk);
+                        const float v = tile_value<T>(sv, r, u % DV, kChunk);
                         if (!(fabsf(v) <= 3.4e38f)) atomicMin(&first_odd, p.reverse ? kChunk - 1 - r : r);
                     }
                     compute_sync();
                     stop = *(volatile int *)&first_odd;
                     void *o = cp.out_f32 ? (void *)(static_cast<float *>(p.o) + out_at)
-                                         : (void *)(static_cast<__nv_bfloat16 *>(p.o) + out_at);
-                    careful_rows<DK, DV>(tile + L::q, sk, sv, state_tile, pw, first, end, stop, p.reverse, inside, p.out,
+                                         : (void *)(static_cast<T *>(p.o) + out_at);
+                    careful_rows<T, DK, DV>(tile + L::q, sk, sv, state_tile, pw, first, end, stop, p.reverse, inside, p.out * state.down,
                                          o, p.ost, p.dv, cp.out_f32);
                     compute_sync();
                     for (int u = tid; u < kChunk * DV; u += kComputeWarps * 32) {
                         const int r = u / DV, col = u % DV;
-                        if (!(fabsf(tile_value(sv, r, col, kChunk)) <= 3.4e38f))
-                            *reinterpret_cast<__nv_bfloat16 *>(sv + tile_byte(r, col, kChunk)) = __float2bfloat16_rn(0.f);
+                        if (!(fabsf(tile_value<T>(sv, r, col, kChunk)) <= 3.4e38f))
+                            *reinterpret_cast<T *>(sv + tile_byte(r, col, kChunk)) = from_float<T>(0.f);
                     }
                     fence_async_shared();
                     arrive(v_ready);
@@ -678,6 +887,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                 const int low = p.reverse ? max(first, kChunk - stop) : first, high = p.reverse ? end : min(end, stop);
                 uint32_t y[COLS];
                 tmem_load(lanes + kY + group * COLS, y);
+                if (HALF) {
+#pragma unroll
+                    for (int j = 0; j < COLS; j++) y[j] = __float_as_uint(__uint_as_float(y[j]) * scores.down);
+                }
                 if (cp.out_f32) {
                     float *o = static_cast<float *>(p.o) + out_at + row * p.ost;
                     if (row >= low && row < high) {
@@ -694,14 +907,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                         uint32_t v[4];
 #pragma unroll
                         for (int e = 0; e < 4; e++)
-                            v[e] = pack_bf16(__uint_as_float(y[k + 2 * e]), __uint_as_float(y[k + 2 * e + 1]));
+                            v[e] = pack<T>(__uint_as_float(y[k + 2 * e]), __uint_as_float(y[k + 2 * e + 1]));
                         *reinterpret_cast<uint4 *>(turn + tile_byte(row, group * COLS + k, kChunk)) =
                             make_uint4(v[0], v[1], v[2], v[3]);
                     }
                     if (!sent) {  // row pieces of the warp's own rows
                         __syncwarp();
                         constexpr int PER = COLS / 8;  // 16-byte pieces of a row
-                        __nv_bfloat16 *o = static_cast<__nv_bfloat16 *>(p.o) + out_at;
+                        T *o = static_cast<T *>(p.o) + out_at;
                         for (int u = 0; u < PER; u++) {
                             const int r = block * 32 + u * (32 / PER) + lane / PER, col = group * COLS + (lane % PER) * 8;
                             if (r >= low && r < high && col < p.dv)
@@ -712,10 +925,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                 }
             }
             if (HALVES == 2) step_state();
-            publish_state();
+            publish_state(c & 1);
             arrive(done + 8 * (c & 1));
         }
-        if (TERMS == 4 && !dead && p.s_out && line.kept && row < p.dk) {
+        if (FINAL && !dead && p.s_out && line.kept && row < p.dk) {
             float *to = p.s_out + line.user + row * p.state_k;
             const bool wide = p.state_v == 1 && (p.dv & 3) == 0 && (reinterpret_cast<uintptr_t>(to) & 15) == 0;
 #pragma unroll
@@ -744,7 +957,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
 #pragma unroll
                     for (int n = 0; n < DK / 16; n++) {
                         const uint32_t at = ((n >> 2) * kPanel + (n & 3) * 32) >> 4;
-                        mma_shared(tmem + kX, q + at, k + at, mma_desc(128, false), n > 0);
+                        mma_shared(tmem + kX, q + at, k + at, mma_desc<T>(128, false), n > 0);
                     }
                     mma_commit(bar_x);
                 };
@@ -759,12 +972,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
 #pragma unroll
                             for (int n = 0; n < 8 / HALVES; n++)
                                 mma_tensor(tmem + kZ, tmem + kW + term * kTermColumns + n * 8, v + ((half * 64 + n * 16) * 128 >> 4),
-                                           mma_desc(DV, true), half > 0 || term > 0 || n > 0);
+                                           mma_desc<T>(DV, true), half > 0 || term > 0 || n > 0);
                     };
                     auto inside_product = [&] {
 #pragma unroll
                         for (int n = 0; n < 8; n++)
-                            mma_tensor(tmem + kY, tmem + kX + (n >> 1) * 32 + (n & 1) * 8, v + (n * 2048 >> 4), mma_desc(DV, true),
+                            mma_tensor(tmem + kY, tmem + kX + (n >> 1) * 32 + (n & 1) * 8, v + (n * 2048 >> 4), mma_desc<T>(DV, true),
                                        true);
                     };
                     // c = 0: the state that enters is in place (every compute warp is done with chunk -1, stage 1)
@@ -774,7 +987,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
 #pragma unroll
                     for (int n = 0; n < DK / 16; n++)
                         mma_shared(tmem + kY, q + (((n >> 2) * kPanel + (n & 3) * 32) >> 4), state + (n * 2048 >> 4),
-                                   mma_desc(DV, true), n > 0);
+                                   mma_desc<T>(DV, true), n > 0);
                     mma_commit(bar_y);
                     barrier_wait(w0_ready, parity, gone);
                     fence_after_sync();
@@ -838,7 +1051,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                     }
             }
         } else {
-            // ---- two warps look for infinities and NaN among the values
+            // ---- two warps look for infinities and NaN among the values, and (f16) for the largest key
             const int which = warp - kComputeWarps - 2;  // half of the rows
             int careful_chunks = 0;
             for (int c = 0; c < chunks; c++) {
@@ -846,16 +1059,24 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                 const int first = p.reverse ? kChunk - n : 0, end = first + n;
                 const unsigned char *sv = smem + (c & 1) * L::stage + L::v + which * 64 * 128 + lane * 16;
                 barrier_wait(full + 8 * (c & 1), (c >> 1) & 1, gone);
+                if (HALF) {  // the compute warps wait for this
+                    const uint32_t most = largest_key<DK>(smem + (c & 1) * L::stage + L::k, which, first, end);
+                    if (lane == 0) {
+                        key_most[which][c & 1] = most;
+                        barrier_arrive(scanned + 8 * (c & 1));
+                    }
+                    __syncwarp();
+                }
                 uint32_t odd = 0;
                 for (int panel = 0; panel < DV / 64; panel++)
 #pragma unroll 4
                     for (int u = 0; u < 16; u++) {  // four rows at a time
                         const uint4 w = *reinterpret_cast<const uint4 *>(sv + panel * kPanel + u * 512);
                         const int r = which * 64 + u * 4 + (lane >> 3);
-                        uint32_t here = (w.x & 0x7f807f80u) + 0x00800080u;
-                        here |= (w.y & 0x7f807f80u) + 0x00800080u;
-                        here |= (w.z & 0x7f807f80u) + 0x00800080u;
-                        here |= (w.w & 0x7f807f80u) + 0x00800080u;
+                        uint32_t here = (w.x & Two<T>::exponent) + Two<T>::above;
+                        here |= (w.y & Two<T>::exponent) + Two<T>::above;
+                        here |= (w.z & Two<T>::exponent) + Two<T>::above;
+                        here |= (w.w & Two<T>::exponent) + Two<T>::above;
                         if (r >= first && r < end) odd |= here;
                     }
                 const bool any = __any_sync(~0u, odd & 0x80008000u);
@@ -938,13 +1159,13 @@ Encode encoder() {
 }
 
 // [dim, heads, tokens, batch] with boxes of 64 x 1 x 128 x 1
-void encode(CUtensorMap &map, const MixOperand &t, const MixParams &p, int dim) {
+void encode(CUtensorMap &map, const MixOperand &t, const MixParams &p, int dim, Element e) {
     const int64_t heads = (p.heads + t.per_head - 1) / t.per_head;
     const int64_t tokens = p.offsets ? p.packed_tokens : p.length, batch = p.offsets ? 1 : p.batch;
     const cuuint64_t size[4] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)tokens, (cuuint64_t)batch};
     const cuuint64_t stride[3] = {(cuuint64_t)t.sh * 2, (cuuint64_t)t.st * 2, (cuuint64_t)(p.offsets ? t.st * 2 : t.sb * 2)};
     const cuuint32_t box[4] = {64, 1, kChunk, 1}, step[4] = {1, 1, 1, 1};
-    const CUresult r = encoder()(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(t.p), size, stride, box, step,
+    const CUresult r = encoder()(&map, e == Element::F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(t.p), size, stride, box, step,
                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) fail_runtime("tensor map encoding failed: error " + std::to_string((int)r));
@@ -977,17 +1198,23 @@ cudaError_t launch(Kernel *kernel, dim3 grid, int threads, int shared, bool afte
     return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
-template <int DK, int DV>
-cudaError_t launch_all(const Maps &maps, const ChunkParams &cp, cudaStream_t s) {
+template <typename T, int DK, int DV>
+cudaError_t launch_dims(const Maps &maps, const ChunkParams &cp, cudaStream_t s) {
     const dim3 grid(cp.count, cp.p.heads, (unsigned)cp.p.batch);
     if (cp.count == 1)  // the state itself is a result (and, wanted or not, it makes the same results)
-        return launch(chunk_kernel<DK, DV, 4>, grid, kThreads, Layout<DK, DV>::dynamic, false, s, maps, cp);
-    cudaError_t e = launch(sum_kernel<DK, DV>, grid, kThreads, SumLayout<DK, DV>::dynamic, false, s, maps, cp);
+        return launch(chunk_kernel<T, DK, DV, true>, grid, kThreads, shared_bytes(Layout<DK, DV>::bytes, sizeof(ChunkSmall)), false, s, maps, cp);
+    cudaError_t e = launch(sum_kernel<T, DK, DV>, grid, kThreads, shared_bytes(SumLayout<DK, DV>::bytes, 0), false, s, maps, cp);
     if (e != cudaSuccess) return e;
     const dim3 elements((cp.p.dk * cp.p.dv + 511) / 512, cp.p.heads, (unsigned)cp.p.batch);
     e = launch(enter_kernel, elements, 128, 0, true, s, cp);
     if (e != cudaSuccess) return e;
-    return launch(chunk_kernel<DK, DV, 2>, grid, kThreads, Layout<DK, DV>::dynamic, true, s, maps, cp);
+    return launch(chunk_kernel<T, DK, DV, false>, grid, kThreads, shared_bytes(Layout<DK, DV>::bytes, sizeof(ChunkSmall)), true, s, maps, cp);
+}
+
+template <typename T>
+cudaError_t launch_type(const Maps &maps, const ChunkParams &cp, cudaStream_t s) {
+    if (cp.p.dk <= 64) return cp.p.dv <= 64 ? launch_dims<T, 64, 64>(maps, cp, s) : launch_dims<T, 64, 128>(maps, cp, s);
+    return cp.p.dv <= 64 ? launch_dims<T, 128, 64>(maps, cp, s) : launch_dims<T, 128, 128>(maps, cp, s);
 }
 
 }  // namespace
@@ -1012,7 +1239,7 @@ Segments segments_of(int64_t length, int64_t batch, int64_t heads) {
 }
 
 bool chunked_tc_takes(const MixParams &p, Element e, bool out_f32) {
-    if (e != Element::BF16 || p.dk > 128 || p.dv > 128 || p.length < 2) return false;
+    if (e == Element::F32 || p.dk > 128 || p.dv > 128 || p.length < 2) return false;
     if (!loadable(p.q, p.dk) || !loadable(p.k, p.dk) || !loadable(p.v, p.dv)) return false;
     const int64_t tokens = p.offsets ? p.packed_tokens : p.length;
     if (tokens == 0 || std::max(tokens, p.length) > int64_t(1) << 30) return false;  // rows are counted in 32 bits
@@ -1021,12 +1248,12 @@ bool chunked_tc_takes(const MixParams &p, Element e, bool out_f32) {
     return stores && encoder();
 }
 
-cudaError_t launch_chunked_tc(const MixParams &p, bool out_f32, float *segments, cudaStream_t s) {
+cudaError_t launch_chunked_tc(const MixParams &p, Element e, bool out_f32, float *segments, cudaStream_t s) {
     Maps maps;
-    encode(maps.q, p.q, p, p.dk);
-    encode(maps.k, p.k, p, p.dk);
-    encode(maps.v, p.v, p, p.dv);
-    if (!out_f32) encode(maps.o, {p.o, p.osb, p.ost, p.osh, 1}, p, p.dv);
+    encode(maps.q, p.q, p, p.dk, e);
+    encode(maps.k, p.k, p, p.dk, e);
+    encode(maps.v, p.v, p, p.dv, e);
+    if (!out_f32) encode(maps.o, {p.o, p.osb, p.ost, p.osh, 1}, p, p.dv, e);
     ChunkParams cp{};
     cp.p = p;
     cp.segments = segments;
@@ -1034,8 +1261,7 @@ cudaError_t launch_chunked_tc(const MixParams &p, bool out_f32, float *segments,
     cp.count = g.count;
     cp.chunks = g.chunks;
     cp.out_f32 = out_f32;
-    if (p.dk <= 64) return p.dv <= 64 ? launch_all<64, 64>(maps, cp, s) : launch_all<64, 128>(maps, cp, s);
-    return p.dv <= 64 ? launch_all<128, 64>(maps, cp, s) : launch_all<128, 128>(maps, cp, s);
+    return e == Element::F16 ? launch_type<__half>(maps, cp, s) : launch_type<__nv_bfloat16>(maps, cp, s);
 }
 
 }  // namespace b200fft

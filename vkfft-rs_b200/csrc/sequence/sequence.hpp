@@ -115,7 +115,7 @@ struct Segments {
 };
 Segments segments_of(int64_t length, int64_t batch, int64_t heads);
 bool chunked_tc_takes(const MixParams &p, Element e, bool out_f32);
-cudaError_t launch_chunked_tc(const MixParams &p, bool out_f32, float *segments, cudaStream_t s);
+cudaError_t launch_chunked_tc(const MixParams &p, Element e, bool out_f32, float *segments, cudaStream_t s);
 
 // dst[.., g, d] = sum over the share query heads of src[token, g * share + j, d]
 struct ShareParams {

@@ -4,6 +4,8 @@
 
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "device.cuh"
 
 namespace b200fft {
@@ -168,10 +170,12 @@ __device__ __forceinline__ uint64_t matrix_desc(uint32_t address, uint32_t leadi
            (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
-// Instruction descriptor of kind::f16 with bf16 operands, f32 results, 128 rows, n columns.
+// Instruction descriptor of kind::f16: operands of type T, f32 results, 128 rows, n columns.
 // b_rows: B's contiguous axis is n and not k.
+template <typename T>
 __host__ __device__ constexpr uint32_t mma_desc(int n, bool b_rows) {
-    return 1u << 4 | 1u << 7 | 1u << 10 | (b_rows ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(128 >> 4) << 24;
+    return 1u << 4 | (std::is_same<T, __nv_bfloat16>::value ? 1u << 7 | 1u << 10 : 0u) | (b_rows ? 1u << 16 : 0u) |
+           (uint32_t)(n >> 3) << 17 | (uint32_t)(128 >> 4) << 24;
 }
 
 __device__ __forceinline__ void mma_shared(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add) {
