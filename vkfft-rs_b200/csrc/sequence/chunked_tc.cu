@@ -20,13 +20,13 @@
 // chunk, from their largest element.  Its two W terms hold 22 bits, f32's own rounding.
 #include <algorithm>
 
+#include "segments.cuh"
 #include "tcgen05.cuh"
 
 namespace b200fft {
 
 namespace {
 
-constexpr int kChunk = 128;
 // 16 warps of arithmetic; a warpgroup in which one thread issues the products, one moves the tiles and two
 // warps look the values over.  (With one thread of the former issuing, its warp held all others up: 5000 of
 // 11700 clocks a chunk.)  640 x 96 registers at launch; afterwards 512 x 104 + 128 x 64.
@@ -38,14 +38,6 @@ constexpr uint32_t kTmemColumns = 512;
 // tensor memory columns: scores and P; results; state update; W terms
 constexpr uint32_t kX = 0, kY = 128, kZ = 256, kW = 384;
 constexpr int kPanel = kChunk * 128;  // bytes of 128 rows x 64 elements
-
-struct ChunkParams {
-    MixParams p;
-    float *segments;  // [batch][heads][count][dk][dv]: first each segment's own sum, then the state that enters it
-    int count;        // segments of a sequence
-    int chunks;       // chunks of a segment
-    int out_f32;
-};
 
 struct Maps {
     CUtensorMap q, k, v, o;
@@ -99,15 +91,6 @@ struct SumLayout {
     static constexpr int stages = 3;
     static constexpr int bytes = stages * stage;
 };
-
-// l s as s + (l - 1) s where l is near one, so that many chunks do not add up l's rounding.
-struct Fade {
-    float whole, rest;
-};
-__device__ __forceinline__ Fade fade_of(double log_l) {
-    return log_l > -0.5 ? Fade{1.f, (float)expm1(log_l)} : Fade{(float)exp(log_l), 0.f};
-}
-__device__ __forceinline__ float faded(float s, Fade f) { return fmaf(s, f.rest, s * f.whole); }
 
 // Byte of column c in row r of a swizzled tile whose panels of 64 columns have `rows` rows.
 __device__ __forceinline__ uint32_t tile_byte(int r, int c, int rows) {
@@ -166,37 +149,6 @@ __device__ __forceinline__ Scale scale_to(float most, int top) {
 
 // Barrier 1: the compute warps among themselves.
 __device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kComputeWarps * 32) : "memory"); }
-// One segment of one head of one sequence.
-struct Line {
-    int start, count;  // rows of the sequence
-    int from, tokens;  // of the segment, in processing order
-    int last;          // the sequence's last segment
-    bool kept;         // has a slot in the state buffers
-    int64_t user;      // its state there
-    __device__ Line(const ChunkParams &cp, int segment, int h, int b) {
-        const MixParams &p = cp.p;
-        const Rows rows = rows_of(p.offsets, p.packed_tokens, p.length, b);
-        start = (int)rows.start;
-        count = (int)rows.count;
-        const int per_segment = cp.chunks * kChunk;
-        last = count > 0 ? (count - 1) / per_segment : 0;
-        from = segment * per_segment;
-        tokens = min(count - from, per_segment);
-        const int64_t slot = p.slots ? p.slots[b] : b;
-        kept = slot >= 0 && slot < p.state_slots;
-        user = (slot * p.heads + h) * (int64_t)p.dk * p.dv;
-    }
-    // first row of chunk c's tile; a tile in reverse ends at the last row not yet done
-    __device__ int first_row(int c, int reverse) const {
-        const int at = from + c * kChunk;
-        return start + (reverse ? count - at - kChunk : at);
-    }
-};
-
-__device__ __forceinline__ float *segment_state(const ChunkParams &cp, int64_t b, int h, int segment) {
-    return cp.segments + ((b * cp.p.heads + h) * cp.count + segment) * (int64_t)cp.p.dk * cp.p.dv;
-}
-
 // The rows of a chunk from the first on whose value holds an infinity or NaN, one by one: the
 // tensor cores' product with a masked score of zero would spread it to tokens before it, so
 // those get the product again without it, and the rest comes from here.  Rare and slow.
@@ -1102,48 +1054,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     if (warp == 0) tmem_free(tmem, kTmemColumns);
 }
 
-// Turns the segments' own sums into the states that enter them, in order, and leaves the final state.
-// Four elements to a thread (dv is a multiple of eight), eight loads in flight.
-__global__ void __launch_bounds__(128) enter_kernel(const __grid_constant__ ChunkParams cp) {
-    constexpr int AHEAD = 8;
-    __shared__ Fade fades[2];
-    const MixParams &p = cp.p;
-    const int h = blockIdx.y, b = blockIdx.z, e = (blockIdx.x * 128 + threadIdx.x) * 4, n = p.dk * p.dv;
-    const Line line(cp, 0, h, b);
-    const int per_segment = cp.chunks * kChunk, last = line.last;
-    if (threadIdx.x < 2)
-        fades[threadIdx.x] = fade_of((double)p.log_decay[h] * (threadIdx.x ? line.count - last * per_segment : per_segment));
-    let_next_start();
-    __syncthreads();
-    if (e >= n) return;
-    const Fade keep = fades[0], keep_last = fades[1];
-    const int64_t user = line.user + (e / p.dv) * p.state_k + (e % p.dv) * p.state_v;
-    wait_for_previous();
-    float s[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) s[i] = p.s_in && line.kept ? p.s_in[user + i * p.state_v] : 0.f;
-    float4 *at = reinterpret_cast<float4 *>(segment_state(cp, b, h, 0) + e);
-    const int step = n / 4;
-    const int sums = p.s_out && line.count > 0 ? last + 1 : last;  // the last segment's is there if someone wants it
-    for (int k0 = 0; k0 <= last; k0 += AHEAD) {
-        float4 sum[AHEAD];
-#pragma unroll
-        for (int k = 0; k < AHEAD; k++) sum[k] = k0 + k < sums ? at[(int64_t)(k0 + k) * step] : make_float4(0, 0, 0, 0);
-#pragma unroll
-        for (int k = 0; k < AHEAD; k++)
-            if (k0 + k <= last) {
-                at[(int64_t)(k0 + k) * step] = make_float4(s[0], s[1], s[2], s[3]);
-                const Fade f = k0 + k < last ? keep : keep_last;
-                s[0] = faded(s[0], f) + sum[k].x, s[1] = faded(s[1], f) + sum[k].y;
-                s[2] = faded(s[2], f) + sum[k].z, s[3] = faded(s[3], f) + sum[k].w;
-            }
-    }
-    if (p.s_out && line.kept) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) p.s_out[user + i * p.state_v] = s[i];
-    }
-}
-
 using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                             const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -1177,27 +1087,6 @@ bool loadable(const MixOperand &t, int dim) {
            t.sh % 8 == 0 && t.sb < widest && t.st < widest && t.sh < widest;
 }
 
-// after: the kernel may start while the one before it ends (it waits for it where it reads its results)
-template <typename Kernel, typename... Args>
-cudaError_t launch(Kernel *kernel, dim3 grid, int threads, int shared, bool after, cudaStream_t s, const Args &...args) {
-    cudaLaunchConfig_t config{};
-    config.gridDim = grid;
-    config.blockDim = dim3(threads);
-    config.dynamicSmemBytes = shared;
-    config.stream = s;
-    cudaLaunchAttribute attribute{};
-    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &attribute;
-    config.numAttrs = after ? 1 : 0;
-    if (shared) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
-        if (e != cudaSuccess) return e;
-    }
-    before_launch();
-    return cudaLaunchKernelEx(&config, kernel, args...);
-}
-
 template <typename T, int DK, int DV>
 cudaError_t launch_dims(const Maps &maps, const ChunkParams &cp, cudaStream_t s) {
     const dim3 grid(cp.count, cp.p.heads, (unsigned)cp.p.batch);
@@ -1205,8 +1094,7 @@ cudaError_t launch_dims(const Maps &maps, const ChunkParams &cp, cudaStream_t s)
         return launch(chunk_kernel<T, DK, DV, true>, grid, kThreads, shared_bytes(Layout<DK, DV>::bytes, sizeof(ChunkSmall)), false, s, maps, cp);
     cudaError_t e = launch(sum_kernel<T, DK, DV>, grid, kThreads, shared_bytes(SumLayout<DK, DV>::bytes, 0), false, s, maps, cp);
     if (e != cudaSuccess) return e;
-    const dim3 elements((cp.p.dk * cp.p.dv + 511) / 512, cp.p.heads, (unsigned)cp.p.batch);
-    e = launch(enter_kernel, elements, 128, 0, true, s, cp);
+    e = launch_enter(cp, s);
     if (e != cudaSuccess) return e;
     return launch(chunk_kernel<T, DK, DV, false>, grid, kThreads, shared_bytes(Layout<DK, DV>::bytes, sizeof(ChunkSmall)), true, s, maps, cp);
 }

@@ -1,0 +1,370 @@
+// Linear attention by chunks of tokens for everything that the tcgen05 kernels do not take: f32, head dimensions up to
+// 256 of any size, any strides and addresses.
+//
+// The same products as there, on tf32 matrix instructions with every f32 operand in two parts of 11 bits: a b = ah bh +
+// ah bl + al bh, off by 2^-22 (16-bit inputs are one part).  A CTA takes 64 value columns of one segment of one head of
+// one sequence; the tile of the state that a warp updates stays in its registers as the accumulator of its products.
+#include <algorithm>
+
+#include "segments.cuh"
+
+namespace b200fft {
+
+namespace {
+
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kSlice = 64;  // value columns of a CTA
+
+// Row pitches in floats that keep the fragments' reads free of bank conflicts: rows by lane / 4 and columns by
+// lane % 4 (pitch 20 mod 32: keys are also read the other way round), and the other way round (8 mod 32).
+constexpr int pitch_by_row(int n) { return n / 32 * 32 + 20; }
+constexpr int pitch_by_column(int n) { return n / 32 * 32 + 8; }
+static_assert(pitch_by_row(32) >= 32 + 4, "pitch");
+
+template <int DK>
+struct BlockLayout {
+    static constexpr int C = DK > 128 ? 32 : 64;  // tokens of a chunk
+    static constexpr int key_pitch = pitch_by_row(DK), value_pitch = pitch_by_column(kSlice), score_pitch = pitch_by_row(C);
+    static constexpr int q = 0, k = q + C * key_pitch, v = k + C * key_pitch, p = v + C * value_pitch,
+                         s = p + C * score_pitch, pw = s + DK * value_pitch, weight = pw + C + 4, end = weight + C;
+    static constexpr int bytes = end * 4;
+};
+
+__device__ __forceinline__ uint32_t to_tf32(float x) {
+    uint32_t r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+    return r;
+}
+// A fragment's elements: the upper 11 bits and, where the element has more, the next 11.
+template <int N, bool WHOLE>
+struct Parts {
+    uint32_t hi[N], lo[WHOLE ? 1 : N];
+    __device__ __forceinline__ void set(int i, float x) {
+        if (WHOLE) {
+            hi[i] = __float_as_uint(x);
+        } else {
+            hi[i] = to_tf32(x);
+            lo[i] = to_tf32(x - __uint_as_float(hi[i]));
+        }
+    }
+};
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+template <bool WA, bool WB>
+__device__ __forceinline__ void multiply(float (&c)[4], const Parts<4, WA> &a, const Parts<2, WB> &b) {
+    if constexpr (!WA) mma_tf32(c, a.lo, b.hi);
+    if constexpr (!WB) mma_tf32(c, a.hi, b.lo);
+    mma_tf32(c, a.hi, b.hi);
+}
+
+// C rows x COLS columns into shared memory as f32; rows outside [first, end) and columns from `cols` on are zero.
+// Tells whether this thread met an infinity or NaN.
+template <typename T, int C, int COLS>
+__device__ __forceinline__ bool load_tile(float *dst, int pitch, const T *src, int64_t stride, int first, int end, int cols) {
+    constexpr int VEC = 16 / sizeof(T);
+    bool odd = false;
+    if (cols % VEC == 0 && stride % VEC == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+        constexpr int PER = COLS / VEC;
+        static_assert(C * PER % kThreads == 0, "whole rounds");
+#pragma unroll 4
+        for (int u = threadIdx.x; u < C * PER; u += kThreads) {
+            const int r = u / PER, c = u % PER * VEC;
+            float f[VEC];
+            if (r >= first && r < end && c < cols) {
+                const uint4 w = *reinterpret_cast<const uint4 *>(src + r * stride + c);
+                const T *e = reinterpret_cast<const T *>(&w);
+#pragma unroll
+                for (int i = 0; i < VEC; i++) f[i] = to_float(e[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; i++) f[i] = 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < VEC; i += 4) {
+                *reinterpret_cast<float4 *>(dst + r * pitch + c + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+                odd |= !(fabsf(f[i]) + fabsf(f[i + 1]) + fabsf(f[i + 2]) + fabsf(f[i + 3]) <= 3.4e38f);
+            }
+        }
+    } else {
+#pragma unroll 8
+        for (int u = threadIdx.x; u < C * COLS; u += kThreads) {
+            const int r = u / COLS, c = u % COLS;
+            const float f = r >= first && r < end && c < cols ? to_float(src[r * stride + c]) : 0.f;
+            dst[r * pitch + c] = f;
+            odd |= !(fabsf(f) <= 3.4e38f);
+        }
+    }
+    return odd;
+}
+
+// SUM: only the segment's own sum of the state, into the workspace.
+template <typename T, typename O, int DK, bool SUM>
+__global__ void __launch_bounds__(kThreads) block_kernel(const __grid_constant__ ChunkParams cp) {
+    using L = BlockLayout<DK>;
+    constexpr int C = L::C;
+    constexpr bool WHOLE = sizeof(T) == 2;                 // the inputs fit one part
+    constexpr int ROW_TILES = C / 16, ACROSS = kWarps / ROW_TILES;
+    constexpr int SCORE_TILES = C / 8 / ACROSS, OUT_TILES = kSlice / 8 / ACROSS;
+    constexpr int STATE_ROWS = DK >= 128 ? DK / 128 : 1;   // 16-row tiles of the state that a warp keeps
+    constexpr int STATE_ACROSS = DK >= 128 ? 1 : 128 / DK, STATE_TILES = kSlice / 8 / STATE_ACROSS;
+    extern __shared__ __align__(16) float shared[];
+    float *const sq = shared + L::q, *const sk = shared + L::k, *const sv = shared + L::v, *const sp = shared + L::p,
+                 *const ss = shared + L::s, *const pw = shared + L::pw, *const weight = shared + L::weight;
+    __shared__ int first_odd;
+
+    const MixParams &p = cp.p;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int slices = (p.dv + kSlice - 1) / kSlice;
+    const int segment = blockIdx.x, h = blockIdx.y / slices, c0 = blockIdx.y % slices * kSlice, b = blockIdx.z;
+    const int cols = min(kSlice, p.dv - c0);
+    const Line line(cp, segment, h, b);
+    if (SUM) let_next_start();
+    if (segment > line.last || (SUM && ((segment == line.last && !p.s_out) || line.count == 0))) return;
+    const int chunks = (line.tokens + C - 1) / C;  // none for an empty sequence, whose state passes through
+    const float log_decay = p.log_decay[h];
+    for (int i = tid; i <= C; i += kThreads) pw[i] = i ? (float)exp((double)log_decay * i) : 1.f;
+
+    // this warp's tile of the state: rows state_row + g, + 8, columns state_col + 8 n + 2 t, + 1
+    const int state_row = warp / STATE_ACROSS * 16 * STATE_ROWS, state_col = warp % STATE_ACROSS * STATE_TILES * 8;
+    float s[STATE_ROWS][STATE_TILES][4];
+    float *const own = segment_state(cp, b, h, segment);
+    if (!SUM) wait_for_previous();
+    const float *in = SUM ? nullptr : cp.count > 1 ? own : p.s_in && line.kept ? p.s_in + line.user : nullptr;
+    float *out = SUM ? own : cp.count == 1 && p.s_out && line.kept ? p.s_out + line.user : nullptr;
+    const int64_t in_k = cp.count > 1 ? p.dv : p.state_k, in_v = cp.count > 1 ? 1 : p.state_v;  // of `out` too
+#pragma unroll
+    for (int m = 0; m < STATE_ROWS; m++)
+#pragma unroll
+        for (int n = 0; n < STATE_TILES; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int r = state_row + 16 * m + g + (e >> 1) * 8, c = state_col + 8 * n + 2 * t + (e & 1);
+                s[m][n][e] = in && r < p.dk && c < cols ? in[r * in_k + (c0 + c) * in_v] : 0.f;
+            }
+    auto publish_state = [&] {
+#pragma unroll
+        for (int m = 0; m < STATE_ROWS; m++)
+#pragma unroll
+            for (int n = 0; n < STATE_TILES; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e += 2)
+                    *reinterpret_cast<float2 *>(ss + (state_row + 16 * m + g + e * 4) * L::value_pitch + state_col + 8 * n + 2 * t) =
+                        make_float2(s[m][n][e], s[m][n][e + 1]);
+    };
+
+    const T *q = static_cast<const T *>(p.q.p) + (p.offsets ? 0 : b * p.q.sb) + (h / p.q.per_head) * p.q.sh;
+    const T *k = static_cast<const T *>(p.k.p) + (p.offsets ? 0 : b * p.k.sb) + (h / p.k.per_head) * p.k.sh;
+    const T *v = static_cast<const T *>(p.v.p) + (p.offsets ? 0 : b * p.v.sb) + (h / p.v.per_head) * p.v.sh + c0;
+    O *o = static_cast<O *>(p.o) + (p.offsets ? 0 : b * p.osb) + h * p.osh + c0;
+    const int row0 = warp / ACROSS * 16;  // of the chunk, for scores and results
+    const float inside = p.update * p.out;
+    int powers_of = 0;
+    Fade keep{1.f, 0.f};
+
+    for (int c = 0; c < chunks; c++) {
+        const int at = line.from + c * C, n = min(C, line.tokens - c * C);
+        const int first = p.reverse ? C - n : 0, end = first + n;  // valid tile rows
+        const int64_t start = line.start + (p.reverse ? line.count - at - C : at);
+        __syncthreads();  // nobody reads the tiles any more
+        if (n != powers_of) {
+            powers_of = n;
+            keep = fade_of((double)log_decay * n);
+            for (int r = tid; r < C; r += kThreads)
+                weight[r] = r >= first && r < end ? p.update * pw[p.reverse ? r + 1 - first : end - 1 - r] : 0.f;
+        }
+        load_tile<T, C, DK>(sk, L::key_pitch, k + start * p.k.st, p.k.st, first, end, p.dk);
+        bool odd = load_tile<T, C, kSlice>(sv, L::value_pitch, v + start * p.v.st, p.v.st, first, end, cols);
+        if (!SUM) {
+            load_tile<T, C, DK>(sq, L::key_pitch, q + start * p.q.st, p.q.st, first, end, p.dk);
+            publish_state();
+        }
+        const bool careful = __syncthreads_or(odd);
+
+        if (!SUM) {
+            // scores
+            float x[SCORE_TILES][4] = {};
+            const int col0 = warp % ACROSS * SCORE_TILES * 8;
+            const bool none = p.reverse ? col0 + SCORE_TILES * 8 <= row0 : col0 >= row0 + 16;
+            if (!none) {
+#pragma unroll 4
+                for (int d = 0; d < DK; d += 8) {
+                    Parts<4, WHOLE> a;
+                    const float *qa = sq + (row0 + g) * L::key_pitch + d + t;
+                    a.set(0, qa[0]), a.set(1, qa[8 * L::key_pitch]), a.set(2, qa[4]), a.set(3, qa[8 * L::key_pitch + 4]);
+#pragma unroll
+                    for (int m = 0; m < SCORE_TILES; m++) {
+                        Parts<2, WHOLE> w;
+                        const float *kb = sk + (col0 + 8 * m + g) * L::key_pitch + d + t;
+                        w.set(0, kb[0]), w.set(1, kb[4]);
+                        multiply(x[m], a, w);
+                    }
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < SCORE_TILES; m++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int i = row0 + g + (e >> 1) * 8, j = col0 + 8 * m + 2 * t + (e & 1), gap = p.reverse ? j - i : i - j;
+                    sp[i * L::score_pitch + j] = gap >= 0 ? x[m][e] * (inside * pw[max(gap, 0)]) : 0.f;
+                }
+        }
+
+        // state
+#pragma unroll
+        for (int m = 0; m < STATE_ROWS; m++)
+#pragma unroll
+            for (int j = 0; j < STATE_TILES; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[m][j][e] = faded(s[m][j][e], keep);
+#pragma unroll 2
+        for (int r = 0; r < C; r += 8) {
+            const float w0 = weight[r + t], w1 = weight[r + t + 4];
+            Parts<4, false> a[STATE_ROWS];
+#pragma unroll
+            for (int m = 0; m < STATE_ROWS; m++) {
+                const float *ka = sk + (r + t) * L::key_pitch + state_row + 16 * m + g;
+                a[m].set(0, ka[0] * w0), a[m].set(1, ka[8] * w0);
+                a[m].set(2, ka[4 * L::key_pitch] * w1), a[m].set(3, ka[4 * L::key_pitch + 8] * w1);
+            }
+#pragma unroll
+            for (int j = 0; j < STATE_TILES; j++) {
+                Parts<2, WHOLE> w;
+                const float *vb = sv + (r + t) * L::value_pitch + state_col + 8 * j + g;
+                w.set(0, vb[0]), w.set(1, vb[4 * L::value_pitch]);
+#pragma unroll
+                for (int m = 0; m < STATE_ROWS; m++) multiply(s[m][j], a[m], w);
+            }
+        }
+        if (SUM) continue;
+        __syncthreads();
+
+        // Infinities and NaN among the values: a masked score of zero times them would spread them to tokens before
+        // them.  The rows from the first of them on are summed one by one; the others' product goes without them.
+        int stop = C;
+        if (careful) {
+            if (tid == 0) first_odd = C;
+            __syncthreads();
+            for (int u = tid; u < C * kSlice; u += kThreads)
+                if (!(fabsf(sv[u / kSlice * L::value_pitch + u % kSlice]) <= 3.4e38f))
+                    atomicMin(&first_odd, p.reverse ? C - 1 - u / kSlice : u / kSlice);
+            __syncthreads();
+            stop = first_odd;
+            for (int u = tid; u < C * kSlice; u += kThreads) {
+                const int i = u / kSlice, col = u % kSlice;
+                if (i < first || i >= end || col >= cols || (p.reverse ? C - 1 - i : i) < stop) continue;
+                float state = 0.f, sum = 0.f;
+                for (int d = 0; d < DK; d++) state = fmaf(sq[i * L::key_pitch + d], ss[d * L::value_pitch + col], state);
+                for (int j = p.reverse ? i : 0; j < (p.reverse ? C : i + 1); j++)
+                    sum = fmaf(sp[i * L::score_pitch + j], sv[j * L::value_pitch + col], sum);
+                o[(start + i) * p.ost + col] = from_float<O>(fmaf(p.out * pw[p.reverse ? C - 1 - i : i + 1], state, sum));
+            }
+            __syncthreads();
+            for (int u = tid; u < C * kSlice; u += kThreads) {
+                float &f = sv[u / kSlice * L::value_pitch + u % kSlice];
+                if (!(fabsf(f) <= 3.4e38f)) f = 0.f;
+            }
+            __syncthreads();
+        }
+
+        // results: the state's part, faded by row, and the part inside the chunk
+        const int col0 = warp % ACROSS * OUT_TILES * 8;
+        float y[OUT_TILES][4] = {};
+#pragma unroll 4
+        for (int d = 0; d < DK; d += 8) {
+            Parts<4, WHOLE> a;
+            const float *qa = sq + (row0 + g) * L::key_pitch + d + t;
+            a.set(0, qa[0]), a.set(1, qa[8 * L::key_pitch]), a.set(2, qa[4]), a.set(3, qa[8 * L::key_pitch + 4]);
+#pragma unroll
+            for (int m = 0; m < OUT_TILES; m++) {
+                Parts<2, false> w;
+                const float *sb = ss + (d + t) * L::value_pitch + col0 + 8 * m + g;
+                w.set(0, sb[0]), w.set(1, sb[4 * L::value_pitch]);
+                multiply(y[m], a, w);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int i = row0 + g + (e >> 1) * 8;
+            const float fade = p.out * pw[p.reverse ? C - 1 - i : i + 1];
+#pragma unroll
+            for (int m = 0; m < OUT_TILES; m++) y[m][e] *= fade;
+        }
+        const int from = p.reverse ? row0 : 0, to = p.reverse ? C : row0 + 16;  // columns of scores that this row tile has
+#pragma unroll 2
+        for (int j = from; j < to; j += 8) {
+            Parts<4, false> a;
+            const float *pa = sp + (row0 + g) * L::score_pitch + j + t;
+            a.set(0, pa[0]), a.set(1, pa[8 * L::score_pitch]), a.set(2, pa[4]), a.set(3, pa[8 * L::score_pitch + 4]);
+#pragma unroll
+            for (int m = 0; m < OUT_TILES; m++) {
+                Parts<2, WHOLE> w;
+                const float *vb = sv + (j + t) * L::value_pitch + col0 + 8 * m + g;
+                w.set(0, vb[0]), w.set(1, vb[4 * L::value_pitch]);
+                multiply(y[m], a, w);
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < OUT_TILES; m++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = row0 + g + (e >> 1) * 8, col = col0 + 8 * m + 2 * t + (e & 1);
+                if (i >= first && i < end && (p.reverse ? C - 1 - i : i) < stop && col < cols)
+                    o[(start + i) * p.ost + col] = from_float<O>(y[m][e]);
+            }
+    }
+
+    if (!out) return;
+#pragma unroll
+    for (int m = 0; m < STATE_ROWS; m++)
+#pragma unroll
+        for (int j = 0; j < STATE_TILES; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int r = state_row + 16 * m + g + (e >> 1) * 8, col = state_col + 8 * j + 2 * t + (e & 1);
+                if (r < p.dk && col < cols) out[r * in_k + (c0 + col) * in_v] = s[m][j][e];
+            }
+}
+
+template <typename T, typename O, int DK>
+cudaError_t launch_dims(const ChunkParams &cp, cudaStream_t s) {
+    const dim3 grid(cp.count, cp.p.heads * ((cp.p.dv + kSlice - 1) / kSlice), (unsigned)cp.p.batch);
+    if (cp.count > 1) {
+        cudaError_t e = launch(block_kernel<T, O, DK, true>, grid, kThreads, BlockLayout<DK>::bytes, false, s, cp);
+        if (e != cudaSuccess) return e;
+        e = launch_enter(cp, s);
+        if (e != cudaSuccess) return e;
+    }
+    return launch(block_kernel<T, O, DK, false>, grid, kThreads, BlockLayout<DK>::bytes, cp.count > 1, s, cp);
+}
+
+template <typename T, typename O>
+cudaError_t launch_type(const ChunkParams &cp, cudaStream_t s) {
+    if (cp.p.dk <= 64) return launch_dims<T, O, 64>(cp, s);
+    return cp.p.dk <= 128 ? launch_dims<T, O, 128>(cp, s) : launch_dims<T, O, 256>(cp, s);
+}
+
+}  // namespace
+
+bool chunked_tf32_takes(const MixParams &p) {
+    const int64_t tokens = p.offsets ? p.packed_tokens : p.length;
+    if ((int64_t)p.heads * ((p.dv + kSlice - 1) / kSlice) > 65535) return false;  // the grid's second axis
+    return p.length >= 2 && tokens > 0 && std::max(tokens, p.length) <= int64_t(1) << 30;  // rows are counted in 32 bits
+}
+
+cudaError_t launch_chunked_tf32(const MixParams &p, Element e, bool out_f32, float *segments, cudaStream_t s) {
+    ChunkParams cp{};
+    cp.p = p;
+    cp.segments = segments;
+    const Segments g = segments_of(p.length, p.batch, p.heads);
+    cp.count = g.count;
+    cp.chunks = g.chunks;
+    return with_element(e, [&](auto v) {
+        using T = decltype(v);
+        return out_f32 ? launch_type<T, float>(cp, s) : launch_type<T, T>(cp, s);
+    });
+}
+
+}  // namespace b200fft

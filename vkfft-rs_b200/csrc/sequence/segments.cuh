@@ -1,0 +1,143 @@
+// Segments of long sequences: what the chunked kernels of linear attention share.
+#pragma once
+
+#include "device.cuh"
+
+namespace b200fft {
+
+namespace {
+
+constexpr int kChunk = 128;  // tokens that segments are counted in
+
+// Programmatic dependent launch: what comes before this may run while the kernel before it ends.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+struct ChunkParams {
+    MixParams p;
+    float *segments;  // [batch][heads][count][dk][dv]: first each segment's own sum, then the state that enters it
+    int count;        // segments of a sequence
+    int chunks;       // chunks of a segment
+    int out_f32;
+};
+
+// l s as s + (l - 1) s where l is near one, so that many chunks do not add up l's rounding.
+struct Fade {
+    float whole, rest;
+};
+__device__ __forceinline__ Fade fade_of(double log_l) {
+    return log_l > -0.5 ? Fade{1.f, (float)expm1(log_l)} : Fade{(float)exp(log_l), 0.f};
+}
+__device__ __forceinline__ float faded(float s, Fade f) { return fmaf(s, f.rest, s * f.whole); }
+
+// One segment of one head of one sequence.
+struct Line {
+    int start, count;  // rows of the sequence
+    int from, tokens;  // of the segment, in processing order
+    int last;          // the sequence's last segment
+    bool kept;         // has a slot in the state buffers
+    int64_t user;      // its state there
+    __device__ Line(const ChunkParams &cp, int segment, int h, int b) {
+        const MixParams &p = cp.p;
+        const Rows rows = rows_of(p.offsets, p.packed_tokens, p.length, b);
+        start = (int)rows.start;
+        count = (int)rows.count;
+        const int per_segment = cp.chunks * kChunk;
+        last = count > 0 ? (count - 1) / per_segment : 0;
+        from = segment * per_segment;
+        tokens = min(count - from, per_segment);
+        const int64_t slot = p.slots ? p.slots[b] : b;
+        kept = slot >= 0 && slot < p.state_slots;
+        user = (slot * p.heads + h) * (int64_t)p.dk * p.dv;
+    }
+    // first row of chunk c's tile; a tile in reverse ends at the last row not yet done
+    __device__ int first_row(int c, int reverse) const {
+        const int at = from + c * kChunk;
+        return start + (reverse ? count - at - kChunk : at);
+    }
+};
+
+__device__ __forceinline__ float *segment_state(const ChunkParams &cp, int64_t b, int h, int segment) {
+    return cp.segments + ((b * cp.p.heads + h) * cp.count + segment) * (int64_t)cp.p.dk * cp.p.dv;
+}
+
+// after: the kernel may start while the one before it ends (it waits for it where it reads its results)
+template <typename Kernel, typename... Args>
+cudaError_t launch(Kernel *kernel, dim3 grid, int threads, int shared, bool after, cudaStream_t s, const Args &...args) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = shared;
+    config.stream = s;
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute;
+    config.numAttrs = after ? 1 : 0;
+    if (shared) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
+        if (e != cudaSuccess) return e;
+    }
+    before_launch();
+    return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
+
+// Turns the segments' own sums into the states that enter them, in order, and leaves the final state.
+// VEC (dv is a multiple of it) elements to a thread, eight loads in flight.
+template <int VEC>
+__global__ void __launch_bounds__(128) enter_kernel(const __grid_constant__ ChunkParams cp) {
+    constexpr int AHEAD = 8;
+    __shared__ Fade fades[2];
+    const MixParams &p = cp.p;
+    const int h = blockIdx.y, b = blockIdx.z, e = (blockIdx.x * 128 + threadIdx.x) * VEC, n = p.dk * p.dv;
+    const Line line(cp, 0, h, b);
+    const int per_segment = cp.chunks * kChunk, last = line.last;
+    if (threadIdx.x < 2)
+        fades[threadIdx.x] = fade_of((double)p.log_decay[h] * (threadIdx.x ? line.count - last * per_segment : per_segment));
+    let_next_start();
+    __syncthreads();
+    if (e >= n) return;
+    const Fade keep = fades[0], keep_last = fades[1];
+    const int64_t user = line.user + (e / p.dv) * p.state_k + (e % p.dv) * p.state_v;
+    wait_for_previous();
+    struct __align__(4 * VEC) Piece {
+        float v[VEC];
+    };
+    Piece s;
+#pragma unroll
+    for (int i = 0; i < VEC; i++) s.v[i] = p.s_in && line.kept ? p.s_in[user + i * p.state_v] : 0.f;
+    Piece *at = reinterpret_cast<Piece *>(segment_state(cp, b, h, 0) + e);
+    const int step = n / VEC;
+    const int sums = p.s_out && line.count > 0 ? last + 1 : last;  // the last segment's is there if someone wants it
+    for (int k0 = 0; k0 <= last; k0 += AHEAD) {
+        Piece sum[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++)
+            if (k0 + k < sums) sum[k] = at[(int64_t)(k0 + k) * step];
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++)
+            if (k0 + k <= last) {
+                at[(int64_t)(k0 + k) * step] = s;
+                if (k0 + k < sums) {
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) s.v[i] = faded(s.v[i], k0 + k < last ? keep : keep_last) + sum[k].v[i];
+                }
+            }
+    }
+    if (p.s_out && line.kept) {
+#pragma unroll
+        for (int i = 0; i < VEC; i++) p.s_out[user + i * p.state_v] = s.v[i];
+    }
+}
+
+// The kernel between a pass that sums the segments up and the pass over them.
+inline cudaError_t launch_enter(const ChunkParams &cp, cudaStream_t s) {
+    const int vec = cp.p.dv % 4 == 0 ? 4 : 1;
+    const dim3 grid((cp.p.dk * cp.p.dv + 128 * vec - 1) / (128 * vec), cp.p.heads, (unsigned)cp.p.batch);
+    return vec == 4 ? launch(enter_kernel<4>, grid, 128, 0, true, s, cp) : launch(enter_kernel<1>, grid, 128, 0, true, s, cp);
+}
+
+}  // namespace
+
+}  // namespace b200fft

@@ -164,6 +164,7 @@ size_t LinearAttention::backward_workspace() const {
 
 static cudaError_t launch_mix(const MixParams &p, Element e, bool out_f32, void *segments, cudaStream_t s) {
     if (p.o && chunked_tc_takes(p, e, out_f32)) return launch_chunked_tc(p, e, out_f32, static_cast<float *>(segments), s);
+    if (p.o && chunked_tf32_takes(p)) return launch_chunked_tf32(p, e, out_f32, static_cast<float *>(segments), s);
     return launch_recurrent(p, e, out_f32, s);
 }
 

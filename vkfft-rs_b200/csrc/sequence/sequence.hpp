@@ -117,6 +117,10 @@ Segments segments_of(int64_t length, int64_t batch, int64_t heads);
 bool chunked_tc_takes(const MixParams &p, Element e, bool out_f32);
 cudaError_t launch_chunked_tc(const MixParams &p, Element e, bool out_f32, float *segments, cudaStream_t s);
 
+// The same for every type, dimension, stride and address, on tf32 matrix instructions.
+bool chunked_tf32_takes(const MixParams &p);
+cudaError_t launch_chunked_tf32(const MixParams &p, Element e, bool out_f32, float *segments, cudaStream_t s);
+
 // dst[.., g, d] = sum over the share query heads of src[token, g * share + j, d]
 struct ShareParams {
     const float *src;  // [tokens][kv_heads * share][dim], token as in the workspace

@@ -199,10 +199,6 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-// Programmatic dependent launch: what comes before this may run while the kernel before it ends.
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 // Registers of a warpgroup.  The shares of all warpgroups together must not exceed what the block was
 // launched with.
 template <int N>
