@@ -270,9 +270,9 @@ __device__ __forceinline__ void clear_rows(unsigned char *tiles, int first, int 
     compute_sync();
 }
 
-// A segment's own sum: what its tokens leave of the state at its end, from a state of zero.  The weights reach to the
-// end of the segment, so that all chunks add up in tensor memory; four terms, as it is an f32 result.  f16, whose keys
-// are scaled by chunk, adds the chunks up in registers instead, one chunk behind the products.
+// A segment's own sum: what its tokens leave of the state at its end, from a state of zero.  Four terms, as it is an
+// f32 result; and the chunks add up in registers, one chunk behind the products: the tensor cores cut sums off where
+// f32 rounds, which over a whole segment would be 2 to 4e-6 of the result, to one side.
 template <typename T, int DK, int DV>
 __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant__ Maps maps,
                                                           const __grid_constant__ ChunkParams cp) {
@@ -280,17 +280,14 @@ __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant_
     constexpr int COLS = DV / kGroups;
     constexpr bool HALF = std::is_same<T, __half>::value;
     constexpr int TERMS = HALF ? 2 : 4;
-    constexpr int kBuffers = 3;                         // of W for half a chunk
-    // columns: W buffers; the sum of all chunks, or of two chunks in turn
-    constexpr uint32_t kW0 = 0, kW1 = HALF ? 64 : 128, kW2 = HALF ? 128 : 384;
-    constexpr uint32_t kSums = 256;
+    constexpr int kBuffers = HALF ? 3 : 2;              // of W for half a chunk
+    constexpr uint32_t kWColumns = TERMS * 32, kSums = 256;  // W buffers from column 0; the products of two chunks in turn
     extern __shared__ unsigned char raw[];
     __shared__ __align__(8) uint64_t bars[3 * L::stages + 2 * kBuffers + 2];
     __shared__ uint32_t tmem_word;
     __shared__ int dead;
     __shared__ float pw[kChunk + 1];  // l^n, times `update` or f16's weight factor
     __shared__ uint32_t key_most[2][L::stages];
-    auto buffer_at = [](int i) { return i == 0 ? kW0 : i == 1 ? kW1 : kW2; };
 
     const MixParams &p = cp.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -304,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant_
     const uint32_t base = shared_address(smem), bar0 = shared_address(bars);
     const uint32_t full = bar0, free = bar0 + 8 * L::stages;                       // tiles have come; are used up
     const uint32_t ready = bar0 + 16 * L::stages, used = ready + 8 * kBuffers;     // W is in place; is used up
-    const uint32_t sums = used + 8 * kBuffers;                                     // a chunk's, or all chunks', products
+    const uint32_t sums = used + 8 * kBuffers;                                     // the products of a chunk
     const uint32_t scanned = sums + 16;                                            // (f16) the keys' largest is known
     if (warp == 0) tmem_alloc(shared_address(&tmem_word), kTmemColumns);
     if (tid == 0) {
@@ -336,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant_
         // reverse: the decay of a row itself; f16 multiplies by it here, as its weights would underflow together
         constexpr int OWN = HALF ? 0 : 1;
         const float factor = p.update * (p.reverse ? expf(log_decay) : 1.f);
-        auto add = [&](int c, int n, float down) {  // f16: s <- l^n s + the products of chunk c
+        auto add = [&](int c, int n, float down) {  // s <- l^n s + the products of chunk c
             barrier_wait(sums + 8 * (c & 1), (c >> 1) & 1, gone);
             fence_after_sync();
             if (row >= DK) return;
@@ -344,14 +341,12 @@ __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant_
             uint32_t x[COLS];
             tmem_load(lanes + kSums + (c & 1) * 128 + group * COLS, x);
 #pragma unroll
-            for (int j = 0; j < COLS; j++) s[j] = fmaf(__uint_as_float(x[j]), down * factor, faded(s[j], keep));
+            for (int j = 0; j < COLS; j++)
+                s[j] = HALF ? fmaf(__uint_as_float(x[j]), down * factor, faded(s[j], keep)) : __uint_as_float(x[j]) + faded(s[j], keep);
         };
         for (int c = 0; c < chunks; c++) {
             const int stage = c % L::stages, n = min(kChunk, line.tokens - c * kChunk);
             const int first = p.reverse ? kChunk - n : 0, end = first + n;
-            // l^(tokens of the segment after this chunk)
-            const int after = HALF ? 0 : max(line.tokens - (c + 1) * kChunk, 0);
-            const float later = expf(log_decay * (float)after);
             barrier_wait(full + 8 * stage, (c / L::stages) & 1, gone);
             if (n < kChunk) clear_rows<L::stage>(smem + stage * L::stage, first, end);
             Scale key{1.f, 1.f};
@@ -371,7 +366,6 @@ __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant_
                     for (int e = 0; e < 2; e++) {
                         const int r = r0 + 8 * pair + e;
                         f[e] = r >= first && r < end ? pw[p.reverse ? r + OWN - first : end - 1 - r] : 0.f;
-                        if (after > 0) f[e] *= later;
                     }
                     split_terms<T, TERMS == 2 ? 2 : 3>(f[0], f[1], &w[0][pair], 2);
                 }
@@ -381,28 +375,20 @@ __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant_
                 }
                 if (row < DK)
                     make_weights<T, TERMS>(keys + stage * L::stage + (half * 4 + group) * 2048, unit, key_factor, w,
-                                    lanes + buffer_at(buffer) + group * 8, 32);
+                                    lanes + buffer * kWColumns + group * 8, 32);
                 tmem_store_wait();
                 fence_before_sync();
                 __syncwarp();
                 if (lane == 0) barrier_arrive(ready + 8 * buffer);
             }
-            if (HALF) {
-                if (c > 0) add(c - 1, kChunk, before.down);
-                before = key;
-            }
+            if (c > 0) add(c - 1, kChunk, before.down);
+            before = key;
         }
-        if (HALF) add(chunks - 1, line.tokens - (chunks - 1) * kChunk, before.down);
-        if (!HALF) barrier_wait(sums, 0, gone);
-        fence_after_sync();
+        add(chunks - 1, line.tokens - (chunks - 1) * kChunk, before.down);
         if (row < DK) {
             uint32_t x[COLS];
-            if (HALF) {
 #pragma unroll
-                for (int j = 0; j < COLS; j++) x[j] = __float_as_uint(s[j]);
-            } else {
-                tmem_load(lanes + kSums + group * COLS, x);
-            }
+            for (int j = 0; j < COLS; j++) x[j] = __float_as_uint(s[j]);
             if (row < p.dk) {
                 float *to = segment_state(cp, b, h, segment) + row * p.dv;
 #pragma unroll
@@ -421,18 +407,20 @@ __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant_
                     const uint64_t v = values + ((base + stage * L::stage + L::v + (i & 1) * 64 * 128) >> 4);
                     barrier_wait(ready + 8 * buffer, (i / kBuffers) & 1, gone);
                     fence_after_sync();
-                    const uint32_t w = tmem + buffer_at(buffer);
+                    const uint32_t w = tmem + buffer * kWColumns;
+                    // the small terms first: sums are cut off in proportion to what has come together
 #pragma unroll
-                    for (int term = 0; term < TERMS; term++)
+                    for (int term = TERMS - 1; term >= 0; term--)
 #pragma unroll
                         for (int n = 0; n < 4; n++)
-                            mma_tensor(tmem + kSums + (HALF ? (i >> 1 & 1) * 128 : 0), w + term * 32 + n * 8, v + (n * 2048 >> 4),
-                                       mma_desc<T>(DV, true), (HALF ? i & 1 : i) > 0 || term > 0 || n > 0);
+                            mma_tensor(tmem + kSums + (i >> 1 & 1) * 128, w + term * 32 + n * 8, v + (n * 2048 >> 4),
+                                       mma_desc<T>(DV, true), (i & 1) > 0 || term < TERMS - 1 || n > 0);
                     mma_commit(used + 8 * buffer);
-                    if (i & 1) mma_commit(free + 8 * stage);
-                    if (HALF && (i & 1)) mma_commit(sums + 8 * (i >> 1 & 1));
+                    if (i & 1) {
+                        mma_commit(free + 8 * stage);
+                        mma_commit(sums + 8 * (i >> 1 & 1));
+                    }
                 }
-                if (!HALF) mma_commit(sums);
             }
         } else if (warp == kComputeWarps + 1) {
             if (lane == 0) {

@@ -53,11 +53,16 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
+// The instruction cuts sums off where f32 rounds; so each eight products are added up by themselves, and to the rest in
+// f32 (added to it by the instruction, 128 of them were off by 2e-6, to one side).
 template <bool WA, bool WB>
 __device__ __forceinline__ void multiply(float (&c)[4], const Parts<4, WA> &a, const Parts<2, WB> &b) {
-    if constexpr (!WA) mma_tf32(c, a.lo, b.hi);
-    if constexpr (!WB) mma_tf32(c, a.hi, b.lo);
-    mma_tf32(c, a.hi, b.hi);
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (!WA) mma_tf32(x, a.lo, b.hi);
+    if constexpr (!WB) mma_tf32(x, a.hi, b.lo);
+    mma_tf32(x, a.hi, b.hi);
+#pragma unroll
+    for (int i = 0; i < 4; i++) c[i] += x[i];
 }
 
 // C rows x COLS columns into shared memory as f32; rows outside [first, end) and columns from `cols` on are zero.
