@@ -1,17 +1,13 @@
 // Segments of long sequences: what the chunked kernels of linear attention share.
 #pragma once
 
-#include "device.cuh"
+#include "launch.cuh"
 
 namespace b200fft {
 
 namespace {
 
 constexpr int kChunk = 128;  // tokens that segments are counted in
-
-// Programmatic dependent launch: what comes before this may run while the kernel before it ends.
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 struct ChunkParams {
     MixParams p;
@@ -60,28 +56,6 @@ struct Line {
 __device__ __forceinline__ float *segment_state(const ChunkParams &cp, int64_t b, int h, int segment) {
     return cp.segments + ((b * cp.p.heads + h) * cp.count + segment) * (int64_t)cp.p.dk * cp.p.dv;
 }
-
-// after: the kernel may start while the one before it ends (it waits for it where it reads its results)
-template <typename Kernel, typename... Args>
-cudaError_t launch(Kernel *kernel, dim3 grid, int threads, int shared, bool after, cudaStream_t s, const Args &...args) {
-    cudaLaunchConfig_t config{};
-    config.gridDim = grid;
-    config.blockDim = dim3(threads);
-    config.dynamicSmemBytes = shared;
-    config.stream = s;
-    cudaLaunchAttribute attribute{};
-    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &attribute;
-    config.numAttrs = after ? 1 : 0;
-    if (shared) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
-        if (e != cudaSuccess) return e;
-    }
-    before_launch();
-    return cudaLaunchKernelEx(&config, kernel, args...);
-}
-
 
 // Turns the segments' own sums into the states that enter them, in order, and leaves the final state.
 // VEC (dv is a multiple of it) elements to a thread, eight loads in flight.

@@ -54,9 +54,12 @@ LayerNorm LayerNorm::from_c(const b200fft_layer_norm_config &c) {
     return n;
 }
 
-int LayerNorm::partials() const { return (int)std::clamp<int64_t>(rows / 64, 1, 64); }
-
-size_t LayerNorm::backward_workspace() const { return (size_t)partials() * features * 2 * sizeof(float); }
+size_t LayerNorm::backward_workspace() const {
+    const int vec = (int)(16 / element_bytes(element));
+    const int groups = std::max(norm_grad_groups(rows, features, 1),
+                                features % vec == 0 ? norm_grad_groups(rows, features, vec) : 1);
+    return (size_t)groups * features * 2 * sizeof(float);
+}
 
 void execute_layer_norm(Context *ctx, const LayerNorm &n, const NormParams &args, cudaStream_t stream) {
     const size_t e = element_bytes(n.element), pe = element_bytes(n.parameter);
@@ -92,12 +95,10 @@ void execute_layer_norm_grad(Context *ctx, const LayerNorm &n, NormGradParams p,
     p.features = n.features;
     p.xs = n.x_stride;
     p.ys = n.y_stride;
-    p.partials = n.partials();
     check(cudaSetDevice(ctx->device), "cudaSetDevice");
     std::lock_guard<std::mutex> l(ctx->mu);
     if (!workspace && (p.dw || p.db)) workspace = context_scratch(ctx, n.backward_workspace());
-    p.part_w = static_cast<float *>(workspace);
-    p.part_b = p.part_w + (size_t)p.partials * n.features;
+    p.part_w = p.dw || p.db ? static_cast<float *>(workspace) : nullptr;
     check(launch_norm_grad(p, n.element, n.parameter, stream ? stream : ctx->stream), "kernel launch");
 }
 

@@ -25,8 +25,7 @@ struct LayerNorm {
     float epsilon;
     Element element, parameter;
     static LayerNorm from_c(const b200fft_layer_norm_config &c);
-    int partials() const;  // row strips whose sums the backward pass keeps apart
-    size_t backward_workspace() const;
+    size_t backward_workspace() const;  // sums of groups of rows that the backward pass keeps apart
 };
 
 struct NormParams {
@@ -36,6 +35,7 @@ struct NormParams {
     int64_t rows, xs, ys;
     int64_t features;
     float epsilon;
+    Element parameter;
 };
 
 struct NormGradParams {
@@ -46,7 +46,10 @@ struct NormGradParams {
     int64_t rows, xs, ys;
     int64_t features;
     int partials;
+    Element parameter;
 };
+// Groups of rows of the backward pass, for accesses of `vec` elements.
+int norm_grad_groups(int64_t rows, int64_t features, int vec);
 
 cudaError_t launch_norm(const NormParams &p, Element e, Element param, cudaStream_t s);
 cudaError_t launch_norm_grad(const NormGradParams &p, Element e, Element param, cudaStream_t s);
