@@ -42,6 +42,10 @@ constexpr int kPanel = kChunk * 128;  // bytes of 128 rows x 64 elements
 struct Maps {
     CUtensorMap q, k, v, o;
 };
+struct TensorPasses {
+    Maps maps[kMostPasses];
+    Passes all;
+};
 
 constexpr int kMostShared = 227 * 1024;  // of a CTA
 
@@ -274,8 +278,7 @@ __device__ __forceinline__ void clear_rows(unsigned char *tiles, int first, int 
 // f32 result; and the chunks add up in registers, one chunk behind the products: the tensor cores cut sums off where
 // f32 rounds, which over a whole segment would be 2 to 4e-6 of the result, to one side.
 template <typename T, int DK, int DV>
-__global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant__ Maps maps,
-                                                          const __grid_constant__ ChunkParams cp) {
+__global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant__ TensorPasses run) {
     using L = SumLayout<DK, DV>;
     constexpr int COLS = DV / kGroups;
     constexpr bool HALF = std::is_same<T, __half>::value;
@@ -289,9 +292,12 @@ __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant_
     __shared__ float pw[kChunk + 1];  // l^n, times `update` or f16's weight factor
     __shared__ uint32_t key_most[2][L::stages];
 
+    const int pass = blockIdx.z / (unsigned)run.all.pass[0].p.batch, b = blockIdx.z % (unsigned)run.all.pass[0].p.batch;
+    const MixPass &cp = run.all.pass[pass];
+    const Maps &maps = run.maps[pass];
     const MixParams &p = cp.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int segment = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+    const int segment = blockIdx.x, h = blockIdx.y;
     const Line line(cp, segment, h, b);
     let_next_start();
     if (segment > line.last || (segment == line.last && !p.s_out) || line.count == 0) return;
@@ -467,16 +473,18 @@ __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant_
 // bf16 terms of the state update's weights: two (2^-17) where the state only goes on into results; four where it is
 // itself a result, in f32: then the weights of half a chunk fill the tensor memory that is left.
 template <typename T, int DK, int DV, bool FINAL>
-__global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constant__ Maps maps,
-                                                            const __grid_constant__ ChunkParams cp) {
+__global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constant__ TensorPasses run) {
     using L = Layout<DK, DV>;
     constexpr int COLS = DV / kGroups;  // state and result columns of one thread
     constexpr bool HALF = std::is_same<T, __half>::value;
     constexpr int TERMS = FINAL && !HALF ? 4 : 2, HALVES = TERMS == 4 ? 2 : 1, kTermColumns = kChunk / 2 / HALVES;
     extern __shared__ unsigned char raw[];
+    const int pass = blockIdx.z / (unsigned)run.all.pass[0].p.batch, b = blockIdx.z % (unsigned)run.all.pass[0].p.batch;
+    const MixPass &cp = run.all.pass[pass];
+    const Maps &maps = run.maps[pass];
     const MixParams &p = cp.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int segment = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+    const int segment = blockIdx.x, h = blockIdx.y;
     const Line line(cp, segment, h, b);
     if (segment > line.last) return;
     const int chunks = (line.tokens + kChunk - 1) / kChunk;
@@ -722,10 +730,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                 }
                 if (HALF) {
                     float most = 0.f;
+                    const uint32_t seen = !on ? ~0u : p.reverse ? ~0u << lane : ~0u >> (31 - lane);  // columns not ahead
                     if (!none) {
 #pragma unroll
                         for (int j = 0; j < 32; j++) {
-                            if (on) x[j] = (p.reverse ? j >= lane : j <= lane) ? x[j] : 0;
+                            // a bit of `seen` as a mask (a choice by comparison became a branch)
+                            x[j] &= (uint32_t)((int32_t)(seen << (31 - j)) >> 31);
                             most = fmaxf(most, fabsf(__uint_as_float(x[j])));
                         }
                     }
@@ -791,7 +801,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
             fence_after_sync();
             {
                 const bool careful = *(volatile int *)&careful_at[c & 1];
-                const bool sent = n == kChunk && !careful && !cp.out_f32;  // whole chunks leave as tiles
+                // whole chunks leave as tiles
+                const bool sent = n == kChunk && !careful && p.o && (!cp.out_f32 || DV <= DK);
                 const int64_t out_at =
                     sent ? 0 : (p.offsets ? 0 : b * p.osb) + h * p.osh + line.first_row(c, p.reverse) * p.ost;
                 int stop = kChunk;  // rows from here on, in processing order, are careful_rows' own
@@ -811,7 +822,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                     stop = *(volatile int *)&first_odd;
                     void *o = cp.out_f32 ? (void *)(static_cast<float *>(p.o) + out_at)
                                          : (void *)(static_cast<T *>(p.o) + out_at);
-                    careful_rows<T, DK, DV>(tile + L::q, sk, sv, state_tile, pw, first, end, stop, p.reverse, inside, p.out * state.down,
+                    if (p.o)
+                        careful_rows<T, DK, DV>(tile + L::q, sk, sv, state_tile, pw, first, end, stop, p.reverse, inside, p.out * state.down,
                                          o, p.ost, p.dv, cp.out_f32);
                     compute_sync();
                     for (int u = tid; u < kChunk * DV; u += kComputeWarps * 32) {
@@ -831,7 +843,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
 #pragma unroll
                     for (int j = 0; j < COLS; j++) y[j] = __float_as_uint(__uint_as_float(y[j]) * scores.down);
                 }
-                if (cp.out_f32) {
+                if (!p.o) {
+                } else if (cp.out_f32 && sent) {
+                    // through shared memory, in the queries' and the keys' place, once every warp has read the keys
+                    barrier_wait(bar_z, parity, gone);
+#pragma unroll
+                    for (int k = 0; k < COLS; k += 4) {
+                        const int col = group * COLS + k;
+                        *reinterpret_cast<uint4 *>(tile + (col >> 5) * kPanel + row * 128 + ((((col >> 2) & 7) ^ (row & 7)) << 4)) =
+                            make_uint4(y[k], y[k + 1], y[k + 2], y[k + 3]);
+                    }
+                } else if (cp.out_f32) {
                     float *o = static_cast<float *>(p.o) + out_at + row * p.ost;
                     if (row >= low && row < high) {
 #pragma unroll
@@ -960,11 +982,18 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                 // the results of chunk c stand in shared memory, unless its threads wrote them themselves
                 auto finish = [&](int c) {
                     barrier_wait(done + 8 * (c & 1), ((c >> 1) + (c & 1)) & 1, gone);
-                    if (cp.out_f32 || dead || *(volatile int *)&careful_at[c & 1] || line.tokens - c * kChunk < kChunk) return;
+                    if (!p.o || (cp.out_f32 && DV > DK) || dead || *(volatile int *)&careful_at[c & 1] ||
+                        line.tokens - c * kChunk < kChunk)
+                        return;
                     const uint32_t src = base + (DV > DK ? L::turn + (c & 1) * (DV / 64) * kPanel : (c & 1) * L::stage + L::q);
                     const int t = line.first_row(c, p.reverse);
-                    for (int n = 0; n < DV / 64; n++)
-                        if (n * 64 < p.dv) tensor_store(&maps.o, src + n * kPanel, n * 64, h, t, bb);
+                    if (cp.out_f32) {
+                        for (int n = 0; n < DV / 32; n++)
+                            if (n * 32 < p.dv) tensor_store(&maps.o, src + n * kPanel, n * 32, h, t, bb);
+                    } else {
+                        for (int n = 0; n < DV / 64; n++)
+                            if (n * 64 < p.dv) tensor_store(&maps.o, src + n * kPanel, n * 64, h, t, bb);
+                    }
                     tensor_store_read();
                 };
                 int c = 0;
@@ -1056,47 +1085,55 @@ Encode encoder() {
     return fn;
 }
 
-// [dim, heads, tokens, batch] with boxes of 64 x 1 x 128 x 1
+// [dim, heads, tokens, batch] with boxes of 128 bytes x 1 x 128 x 1
 void encode(CUtensorMap &map, const MixOperand &t, const MixParams &p, int dim, Element e) {
-    const int64_t heads = (p.heads + t.per_head - 1) / t.per_head;
+    const int64_t heads = (p.heads + t.per_head - 1) / t.per_head, size_of = element_bytes(e);
     const int64_t tokens = p.offsets ? p.packed_tokens : p.length, batch = p.offsets ? 1 : p.batch;
     const cuuint64_t size[4] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)tokens, (cuuint64_t)batch};
-    const cuuint64_t stride[3] = {(cuuint64_t)t.sh * 2, (cuuint64_t)t.st * 2, (cuuint64_t)(p.offsets ? t.st * 2 : t.sb * 2)};
-    const cuuint32_t box[4] = {64, 1, kChunk, 1}, step[4] = {1, 1, 1, 1};
-    const CUresult r = encoder()(&map, e == Element::F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(t.p), size, stride, box, step,
+    const cuuint64_t stride[3] = {(cuuint64_t)(t.sh * size_of), (cuuint64_t)(t.st * size_of),
+                                  (cuuint64_t)((p.offsets ? t.st : t.sb) * size_of)};
+    const cuuint32_t box[4] = {(cuuint32_t)(128 / size_of), 1, kChunk, 1}, step[4] = {1, 1, 1, 1};
+    const CUtensorMapDataType type = e == Element::F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : e == Element::F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                         : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const CUresult r = encoder()(&map, type, 4, const_cast<void *>(t.p), size, stride, box, step,
                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) fail_runtime("tensor map encoding failed: error " + std::to_string((int)r));
 }
 
 bool loadable(const MixOperand &t, int dim) {
-    const int64_t widest = int64_t(1) << 38;  // strides stay below 2^40 bytes
+    const int64_t widest = int64_t(1) << 37;  // strides stay below 2^40 bytes
     return dim % 8 == 0 && (reinterpret_cast<uintptr_t>(t.p) & 15) == 0 && t.sb % 8 == 0 && t.st % 8 == 0 &&
            t.sh % 8 == 0 && t.sb < widest && t.st < widest && t.sh < widest;
 }
 
 template <typename T, int DK, int DV>
-cudaError_t launch_dims(const Maps &maps, const ChunkParams &cp, cudaStream_t s) {
-    const dim3 grid(cp.count, cp.p.heads, (unsigned)cp.p.batch);
-    if (cp.count == 1)  // the state itself is a result (and, wanted or not, it makes the same results)
-        return launch(chunk_kernel<T, DK, DV, true>, grid, kThreads, shared_bytes(Layout<DK, DV>::bytes, sizeof(ChunkSmall)), false, s, maps, cp);
-    cudaError_t e = launch(sum_kernel<T, DK, DV>, grid, kThreads, shared_bytes(SumLayout<DK, DV>::bytes, 0), false, s, maps, cp);
+cudaError_t launch_dims(const TensorPasses &run, int passes, cudaStream_t s) {
+    const MixPass &first = run.all.pass[0];
+    const dim3 grid(first.count, first.p.heads, (unsigned)first.p.batch * passes);
+    if (first.count == 1)  // the state itself is a result (and, wanted or not, it makes the same results)
+        return launch(chunk_kernel<T, DK, DV, true>, grid, kThreads, shared_bytes(Layout<DK, DV>::bytes, sizeof(ChunkSmall)), false, s, run);
+    cudaError_t e = launch(sum_kernel<T, DK, DV>, grid, kThreads, shared_bytes(SumLayout<DK, DV>::bytes, 0), false, s, run);
+    if (e == cudaSuccess) e = launch_enter(run.all, passes, s);
     if (e != cudaSuccess) return e;
-    e = launch_enter(cp, s);
-    if (e != cudaSuccess) return e;
-    return launch(chunk_kernel<T, DK, DV, false>, grid, kThreads, shared_bytes(Layout<DK, DV>::bytes, sizeof(ChunkSmall)), true, s, maps, cp);
+    return launch(chunk_kernel<T, DK, DV, false>, grid, kThreads, shared_bytes(Layout<DK, DV>::bytes, sizeof(ChunkSmall)), true, s, run);
 }
 
 template <typename T>
-cudaError_t launch_type(const Maps &maps, const ChunkParams &cp, cudaStream_t s) {
-    if (cp.p.dk <= 64) return cp.p.dv <= 64 ? launch_dims<T, 64, 64>(maps, cp, s) : launch_dims<T, 64, 128>(maps, cp, s);
-    return cp.p.dv <= 64 ? launch_dims<T, 128, 64>(maps, cp, s) : launch_dims<T, 128, 128>(maps, cp, s);
+cudaError_t launch_type(const TensorPasses &run, int passes, cudaStream_t s) {
+    switch (chunked_tc_shape(run.all.pass[0])) {
+        case 0: return launch_dims<T, 64, 64>(run, passes, s);
+        case 1: return launch_dims<T, 64, 128>(run, passes, s);
+        case 2: return launch_dims<T, 128, 64>(run, passes, s);
+        default: return launch_dims<T, 128, 128>(run, passes, s);
+    }
 }
 
 }  // namespace
 
-Segments segments_of(int64_t length, int64_t batch, int64_t heads) {
-    const int64_t chunks = (length + kChunk - 1) / kChunk, lines = batch * heads;
+Segments segments_of(int64_t length, int64_t lines) {
+    const int64_t chunks = (length + kChunk - 1) / kChunk;
     // microseconds: waves of CTAs, each with its start and its chunks.  One segment: 3.5 a chunk (four terms);
     // more: 3.1 and 1.6 for the pass before it, twice the start, and the kernel between the two.
     Segments best{1, (int)chunks};
@@ -1114,30 +1151,28 @@ Segments segments_of(int64_t length, int64_t batch, int64_t heads) {
     return best;
 }
 
-bool chunked_tc_takes(const MixParams &p, Element e, bool out_f32) {
+int chunked_tc_shape(const MixPass &pass) { return (pass.p.dk > 64 ? 2 : 0) + (pass.p.dv > 64 ? 1 : 0); }
+
+bool chunked_tc_takes(const MixPass &pass, Element e) {
+    const MixParams &p = pass.p;
     if (e == Element::F32 || p.dk > 128 || p.dv > 128 || p.length < 2) return false;
     if (!loadable(p.q, p.dk) || !loadable(p.k, p.dk) || !loadable(p.v, p.dv)) return false;
     const int64_t tokens = p.offsets ? p.packed_tokens : p.length;
     if (tokens == 0 || std::max(tokens, p.length) > int64_t(1) << 30) return false;  // rows are counted in 32 bits
-    const bool stores = out_f32 ? (reinterpret_cast<uintptr_t>(p.o) & 15) == 0 && p.osb % 4 == 0 && p.ost % 4 == 0 && p.osh % 4 == 0
-                                : loadable({p.o, p.osb, p.ost, p.osh, 1}, p.dv);
-    return stores && encoder();
+    return loadable({p.o, p.osb, p.ost, p.osh, 1}, p.dv) && encoder();
 }
 
-cudaError_t launch_chunked_tc(const MixParams &p, Element e, bool out_f32, float *segments, cudaStream_t s) {
-    Maps maps;
-    encode(maps.q, p.q, p, p.dk, e);
-    encode(maps.k, p.k, p, p.dk, e);
-    encode(maps.v, p.v, p, p.dv, e);
-    if (!out_f32) encode(maps.o, {p.o, p.osb, p.ost, p.osh, 1}, p, p.dv, e);
-    ChunkParams cp{};
-    cp.p = p;
-    cp.segments = segments;
-    const Segments g = segments_of(p.length, p.batch, p.heads);
-    cp.count = g.count;
-    cp.chunks = g.chunks;
-    cp.out_f32 = out_f32;
-    return e == Element::F16 ? launch_type<__half>(maps, cp, s) : launch_type<__nv_bfloat16>(maps, cp, s);
+cudaError_t launch_chunked_tc(const MixPass *passes, int n, Element e, cudaStream_t s) {
+    TensorPasses run{};
+    for (int k = 0; k < n; k++) {
+        const MixParams &p = passes[k].p;
+        run.all.pass[k] = passes[k];
+        encode(run.maps[k].q, p.q, p, p.dk, e);
+        encode(run.maps[k].k, p.k, p, p.dk, e);
+        encode(run.maps[k].v, p.v, p, p.dv, e);
+        if (p.o) encode(run.maps[k].o, {p.o, p.osb, p.ost, p.osh, 1}, p, p.dv, passes[k].out_f32 ? Element::F32 : e);
+    }
+    return e == Element::F16 ? launch_type<__half>(run, n, s) : launch_type<__nv_bfloat16>(run, n, s);
 }
 
 }  // namespace b200fft

@@ -106,8 +106,8 @@ __device__ __forceinline__ bool load_tile(float *dst, int pitch, const T *src, i
 }
 
 // SUM: only the segment's own sum of the state, into the workspace.
-template <typename T, typename O, int DK, bool SUM>
-__global__ void __launch_bounds__(kThreads) block_kernel(const __grid_constant__ ChunkParams cp) {
+template <typename T, int DK, bool SUM>
+__global__ void __launch_bounds__(kThreads) block_kernel(const __grid_constant__ Passes all) {
     using L = BlockLayout<DK>;
     constexpr int C = L::C;
     constexpr bool WHOLE = sizeof(T) == 2;                 // the inputs fit one part
@@ -120,10 +120,13 @@ __global__ void __launch_bounds__(kThreads) block_kernel(const __grid_constant__
                  *const ss = shared + L::s, *const pw = shared + L::pw, *const weight = shared + L::weight;
     __shared__ int first_odd;
 
+    const int b = blockIdx.z % (unsigned)all.pass[0].p.batch;
+    const MixPass &cp = all.pass[blockIdx.z / (unsigned)all.pass[0].p.batch];
     const MixParams &p = cp.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int slices = (p.dv + kSlice - 1) / kSlice;
-    const int segment = blockIdx.x, h = blockIdx.y / slices, c0 = blockIdx.y % slices * kSlice, b = blockIdx.z;
+    const int slices = gridDim.y / p.heads;
+    const int segment = blockIdx.x, h = blockIdx.y / slices, c0 = blockIdx.y % slices * kSlice;
+    if (c0 >= p.dv) return;  // the widest pass decides the grid
     const int cols = min(kSlice, p.dv - c0);
     const Line line(cp, segment, h, b);
     if (SUM) let_next_start();
@@ -163,7 +166,13 @@ __global__ void __launch_bounds__(kThreads) block_kernel(const __grid_constant__
     const T *q = static_cast<const T *>(p.q.p) + (p.offsets ? 0 : b * p.q.sb) + (h / p.q.per_head) * p.q.sh;
     const T *k = static_cast<const T *>(p.k.p) + (p.offsets ? 0 : b * p.k.sb) + (h / p.k.per_head) * p.k.sh;
     const T *v = static_cast<const T *>(p.v.p) + (p.offsets ? 0 : b * p.v.sb) + (h / p.v.per_head) * p.v.sh + c0;
-    O *o = static_cast<O *>(p.o) + (p.offsets ? 0 : b * p.osb) + h * p.osh + c0;
+    const int64_t out_at = (p.offsets ? 0 : b * p.osb) + h * p.osh + c0;
+    auto write = [&](int64_t row, int col, float y) {
+        if (cp.out_f32)
+            static_cast<float *>(p.o)[out_at + row * p.ost + col] = y;
+        else
+            static_cast<T *>(p.o)[out_at + row * p.ost + col] = from_float<T>(y);
+    };
     const int row0 = warp / ACROSS * 16;  // of the chunk, for scores and results
     const float inside = p.update * p.out;
     int powers_of = 0;
@@ -264,7 +273,7 @@ __global__ void __launch_bounds__(kThreads) block_kernel(const __grid_constant__
                 for (int d = 0; d < DK; d++) state = fmaf(sq[i * L::key_pitch + d], ss[d * L::value_pitch + col], state);
                 for (int j = p.reverse ? i : 0; j < (p.reverse ? C : i + 1); j++)
                     sum = fmaf(sp[i * L::score_pitch + j], sv[j * L::value_pitch + col], sum);
-                o[(start + i) * p.ost + col] = from_float<O>(fmaf(p.out * pw[p.reverse ? C - 1 - i : i + 1], state, sum));
+                if (p.o) write(start + i, col, fmaf(p.out * pw[p.reverse ? C - 1 - i : i + 1], state, sum));
             }
             __syncthreads();
             for (int u = tid; u < C * kSlice; u += kThreads) {
@@ -316,8 +325,7 @@ __global__ void __launch_bounds__(kThreads) block_kernel(const __grid_constant__
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int i = row0 + g + (e >> 1) * 8, col = col0 + 8 * m + 2 * t + (e & 1);
-                if (i >= first && i < end && (p.reverse ? C - 1 - i : i) < stop && col < cols)
-                    o[(start + i) * p.ost + col] = from_float<O>(y[m][e]);
+                if (p.o && i >= first && i < end && (p.reverse ? C - 1 - i : i) < stop && col < cols) write(start + i, col, y[m][e]);
             }
     }
 
@@ -333,42 +341,41 @@ __global__ void __launch_bounds__(kThreads) block_kernel(const __grid_constant__
             }
 }
 
-template <typename T, typename O, int DK>
-cudaError_t launch_dims(const ChunkParams &cp, cudaStream_t s) {
-    const dim3 grid(cp.count, cp.p.heads * ((cp.p.dv + kSlice - 1) / kSlice), (unsigned)cp.p.batch);
-    if (cp.count > 1) {
-        cudaError_t e = launch(block_kernel<T, O, DK, true>, grid, kThreads, BlockLayout<DK>::bytes, false, s, cp);
-        if (e != cudaSuccess) return e;
-        e = launch_enter(cp, s);
+template <typename T, int DK>
+cudaError_t launch_dims(const Passes &all, int passes, cudaStream_t s) {
+    const MixPass &first = all.pass[0];
+    int slices = 1;
+    for (int k = 0; k < passes; k++) slices = std::max(slices, (all.pass[k].p.dv + kSlice - 1) / kSlice);
+    const dim3 grid(first.count, first.p.heads * slices, (unsigned)first.p.batch * passes);
+    if (first.count > 1) {
+        cudaError_t e = launch(block_kernel<T, DK, true>, grid, kThreads, BlockLayout<DK>::bytes, false, s, all);
+        if (e == cudaSuccess) e = launch_enter(all, passes, s);
         if (e != cudaSuccess) return e;
     }
-    return launch(block_kernel<T, O, DK, false>, grid, kThreads, BlockLayout<DK>::bytes, cp.count > 1, s, cp);
-}
-
-template <typename T, typename O>
-cudaError_t launch_type(const ChunkParams &cp, cudaStream_t s) {
-    if (cp.p.dk <= 64) return launch_dims<T, O, 64>(cp, s);
-    return cp.p.dk <= 128 ? launch_dims<T, O, 128>(cp, s) : launch_dims<T, O, 256>(cp, s);
+    return launch(block_kernel<T, DK, false>, grid, kThreads, BlockLayout<DK>::bytes, first.count > 1, s, all);
 }
 
 }  // namespace
 
-bool chunked_tf32_takes(const MixParams &p) {
+bool chunked_tf32_takes(const MixPass &pass) {
+    const MixParams &p = pass.p;
     const int64_t tokens = p.offsets ? p.packed_tokens : p.length;
-    if ((int64_t)p.heads * ((p.dv + kSlice - 1) / kSlice) > 65535) return false;  // the grid's second axis
+    if ((int64_t)p.heads * 4 > 65535) return false;  // the grid's second axis: up to four slices of a head
     return p.length >= 2 && tokens > 0 && std::max(tokens, p.length) <= int64_t(1) << 30;  // rows are counted in 32 bits
 }
 
-cudaError_t launch_chunked_tf32(const MixParams &p, Element e, bool out_f32, float *segments, cudaStream_t s) {
-    ChunkParams cp{};
-    cp.p = p;
-    cp.segments = segments;
-    const Segments g = segments_of(p.length, p.batch, p.heads);
-    cp.count = g.count;
-    cp.chunks = g.chunks;
+int chunked_tf32_shape(const MixPass &pass) { return pass.p.dk <= 64 ? 64 : pass.p.dk <= 128 ? 128 : 256; }
+
+cudaError_t launch_chunked_tf32(const MixPass *passes, int n, Element e, cudaStream_t s) {
+    Passes all{};
+    for (int k = 0; k < n; k++) all.pass[k] = passes[k];
     return with_element(e, [&](auto v) {
         using T = decltype(v);
-        return out_f32 ? launch_type<T, float>(cp, s) : launch_type<T, T>(cp, s);
+        switch (chunked_tf32_shape(passes[0])) {
+            case 64: return launch_dims<T, 64>(all, n, s);
+            case 128: return launch_dims<T, 128>(all, n, s);
+            default: return launch_dims<T, 256>(all, n, s);
+        }
     });
 }
 

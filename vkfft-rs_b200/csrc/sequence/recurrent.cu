@@ -120,40 +120,69 @@ cudaError_t launch_typed(const MixParams &p, cudaStream_t s) {
     return cudaGetLastError();
 }
 
-// Sums the partial gradients of the query heads that share a key/value head, in head order.
-template <typename T>
-__global__ void __launch_bounds__(256) share_kernel(ShareParams p) {
+// Sums the partial gradients of the query heads that share a key/value head, in head order: VEC dimensions to a
+// thread, kTokens tokens to a block.
+constexpr int kTokens = 8;
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) share_kernel(const __grid_constant__ ShareParams p) {
+    const ShareTensor &t = p.tensor[blockIdx.z];
     const int64_t b = blockIdx.y;
     const Rows rows = rows_of(p.offsets, p.packed_tokens, p.length, b);
-    const int64_t per = (int64_t)p.kv_heads * p.dim, n = rows.count * per;
-    const int64_t first = rows.start + (p.offsets ? 0 : b * p.length);
-    T *dst = static_cast<T *>(p.dst) + (p.offsets ? 0 : b * p.sb);
-    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t t = i / per;
-        const int r = (int)(i - t * per), g = r / p.dim, d = r - g * p.dim;
-        const float *src = p.src + ((first + t) * p.kv_heads + g) * p.share * (int64_t)p.dim + d;
-        float s = 0;
-        for (int j = 0; j < p.share; j++) s += src[j * p.dim];
-        dst[(rows.start + t) * p.st + g * p.sh + d] = from_float<T>(s);
+    const int64_t token0 = (int64_t)blockIdx.x * kTokens;
+    const int tokens = (int)min((int64_t)kTokens, rows.count - token0);
+    const int units = t.dim / VEC, per = p.kv_heads * units;
+    const float *src = t.src + (rows.start + (p.offsets ? 0 : b * p.length) + token0) * p.kv_heads * p.share * (int64_t)t.dim;
+    T *dst = static_cast<T *>(t.dst) + (p.offsets ? 0 : b * t.sb) + (rows.start + token0) * t.st;
+    for (int i = threadIdx.x; i < tokens * per; i += 256) {
+        const int token = i / per, r = i - token * per, g = r / units, d = (r - g * units) * VEC;
+        const float *from = src + ((int64_t)token * p.kv_heads + g) * p.share * t.dim + d;
+        float s[VEC] = {};
+        for (int j = 0; j < p.share; j++) {
+            if constexpr (VEC == 4) {
+                const float4 v = *reinterpret_cast<const float4 *>(from + (int64_t)j * t.dim);
+                s[0] += v.x, s[1] += v.y, s[2] += v.z, s[3] += v.w;
+            } else {
+                s[0] += from[(int64_t)j * t.dim];
+            }
+        }
+        T *to = dst + token * t.st + g * t.sh + d;
+        if constexpr (VEC == 4) {
+            struct __align__(4 * sizeof(T)) Piece {
+                T v[4];
+            } piece;
+#pragma unroll
+            for (int e = 0; e < 4; e++) piece.v[e] = from_float<T>(s[e]);
+            *reinterpret_cast<Piece *>(to) = piece;
+        } else {
+            *to = from_float<T>(s[0]);
+        }
     }
 }
 
 }  // namespace
 
-cudaError_t launch_recurrent(const MixParams &p, Element e, bool out_f32, cudaStream_t s) {
+cudaError_t launch_recurrent(const MixPass &pass, Element e, cudaStream_t s) {
     return with_element(e, [&](auto t) {
         using T = decltype(t);
-        return out_f32 ? launch_typed<T, float>(p, s) : launch_typed<T, T>(p, s);
+        return pass.out_f32 ? launch_typed<T, float>(pass.p, s) : launch_typed<T, T>(pass.p, s);
     });
 }
 
-cudaError_t launch_share(const ShareParams &p, Element e, cudaStream_t s) {
-    return with_element(e, [&](auto t) {
-        using T = decltype(t);
-        const int64_t n = p.length * p.kv_heads * p.dim;
-        const dim3 grid((unsigned)std::min<int64_t>((n + 255) / 256, 4096), (unsigned)p.batch);
+cudaError_t launch_share(const ShareParams &p, int tensors, Element e, cudaStream_t s) {
+    bool four = true;
+    for (int k = 0; k < tensors; k++) {
+        const ShareTensor &t = p.tensor[k];
+        four = four && t.dim % 4 == 0 && (t.sb | t.st | t.sh) % 4 == 0 &&
+               reinterpret_cast<uintptr_t>(t.dst) % (4 * element_bytes(e)) == 0 && (reinterpret_cast<uintptr_t>(t.src) & 15) == 0;
+    }
+    return with_element(e, [&](auto v) {
+        using T = decltype(v);
+        const dim3 grid((unsigned)((p.length + kTokens - 1) / kTokens), (unsigned)p.batch, (unsigned)tensors);
         before_launch();
-        share_kernel<T><<<grid, 256, 0, s>>>(p);
+        if (four)
+            share_kernel<T, 4><<<grid, 256, 0, s>>>(p);
+        else
+            share_kernel<T, 1><<<grid, 256, 0, s>>>(p);
         return cudaGetLastError();
     });
 }

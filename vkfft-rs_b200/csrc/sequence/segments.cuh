@@ -9,12 +9,8 @@ namespace {
 
 constexpr int kChunk = 128;  // tokens that segments are counted in
 
-struct ChunkParams {
-    MixParams p;
-    float *segments;  // [batch][heads][count][dk][dv]: first each segment's own sum, then the state that enters it
-    int count;        // segments of a sequence
-    int chunks;       // chunks of a segment
-    int out_f32;
+struct Passes {
+    MixPass pass[kMostPasses];
 };
 
 // l s as s + (l - 1) s where l is near one, so that many chunks do not add up l's rounding.
@@ -33,7 +29,7 @@ struct Line {
     int last;          // the sequence's last segment
     bool kept;         // has a slot in the state buffers
     int64_t user;      // its state there
-    __device__ Line(const ChunkParams &cp, int segment, int h, int b) {
+    __device__ Line(const MixPass &cp, int segment, int h, int b) {
         const MixParams &p = cp.p;
         const Rows rows = rows_of(p.offsets, p.packed_tokens, p.length, b);
         start = (int)rows.start;
@@ -53,18 +49,20 @@ struct Line {
     }
 };
 
-__device__ __forceinline__ float *segment_state(const ChunkParams &cp, int64_t b, int h, int segment) {
+__device__ __forceinline__ float *segment_state(const MixPass &cp, int64_t b, int h, int segment) {
     return cp.segments + ((b * cp.p.heads + h) * cp.count + segment) * (int64_t)cp.p.dk * cp.p.dv;
 }
 
 // Turns the segments' own sums into the states that enter them, in order, and leaves the final state.
 // VEC (dv is a multiple of it) elements to a thread, eight loads in flight.
 template <int VEC>
-__global__ void __launch_bounds__(128) enter_kernel(const __grid_constant__ ChunkParams cp) {
+__global__ void __launch_bounds__(128) enter_kernel(const __grid_constant__ Passes all) {
     constexpr int AHEAD = 8;
     __shared__ Fade fades[2];
+    const int b = (int)(blockIdx.z % all.pass[0].p.batch);
+    const MixPass &cp = all.pass[blockIdx.z / all.pass[0].p.batch];
     const MixParams &p = cp.p;
-    const int h = blockIdx.y, b = blockIdx.z, e = (blockIdx.x * 128 + threadIdx.x) * VEC, n = p.dk * p.dv;
+    const int h = blockIdx.y, e = (blockIdx.x * 128 + threadIdx.x) * VEC, n = p.dk * p.dv;
     const Line line(cp, 0, h, b);
     const int per_segment = cp.chunks * kChunk, last = line.last;
     if (threadIdx.x < 2)
@@ -106,10 +104,13 @@ __global__ void __launch_bounds__(128) enter_kernel(const __grid_constant__ Chun
 }
 
 // The kernel between a pass that sums the segments up and the pass over them.
-inline cudaError_t launch_enter(const ChunkParams &cp, cudaStream_t s) {
-    const int vec = cp.p.dv % 4 == 0 ? 4 : 1;
-    const dim3 grid((cp.p.dk * cp.p.dv + 128 * vec - 1) / (128 * vec), cp.p.heads, (unsigned)cp.p.batch);
-    return vec == 4 ? launch(enter_kernel<4>, grid, 128, 0, true, s, cp) : launch(enter_kernel<1>, grid, 128, 0, true, s, cp);
+inline cudaError_t launch_enter(const Passes &all, int passes, cudaStream_t s) {
+    const MixParams &p = all.pass[0].p;
+    bool four = true;  // the passes' states have the same size; their rows need not
+    for (int k = 0; k < passes; k++) four = four && all.pass[k].p.dv % 4 == 0;
+    const int vec = four ? 4 : 1;
+    const dim3 grid((p.dk * p.dv + 128 * vec - 1) / (128 * vec), p.heads, (unsigned)p.batch * passes);
+    return four ? launch(enter_kernel<4>, grid, 128, 0, true, s, all) : launch(enter_kernel<1>, grid, 128, 0, true, s, all);
 }
 
 }  // namespace

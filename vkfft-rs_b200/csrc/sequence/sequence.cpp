@@ -152,27 +152,59 @@ LinearAttention LinearAttention::from_c(const b200fft_linear_attention_config &c
     return a;
 }
 
-size_t LinearAttention::segment_bytes() const {
-    if (length < 2) return 0;
-    const Segments g = segments_of(length, batch, heads);
+// The passes of one call run side by side; how a sequence is cut goes by all of them, wanted or not, so that the bits of
+// one gradient do not depend on which others are asked for.
+Segments LinearAttention::segments(int passes) const {
+    return length < 2 ? Segments{1, 1} : segments_of(length, batch * heads * passes);
+}
+
+size_t LinearAttention::segment_bytes(int passes) const {
+    const Segments g = segments(passes);
     return g.count > 1 ? (size_t)batch * heads * g.count * key_dim * value_dim * sizeof(float) : 0;
 }
 
 size_t LinearAttention::backward_workspace() const {
     // the segments' states, and f32 partial gradients of every query head where key/value heads are shared
-    return segment_bytes() + (share() > 1 ? (size_t)tokens() * heads * (key_dim + value_dim) * sizeof(float) : 0);
+    return kMostPasses * segment_bytes(kMostPasses) +
+           (share() > 1 ? (size_t)tokens() * heads * (key_dim + value_dim) * sizeof(float) : 0);
 }
 
-static cudaError_t launch_mix(const MixParams &p, Element e, bool out_f32, void *segments, cudaStream_t s) {
-    if (p.o && chunked_tc_takes(p, e, out_f32)) return launch_chunked_tc(p, e, out_f32, static_cast<float *>(segments), s);
-    if (p.o && chunked_tf32_takes(p)) return launch_chunked_tf32(p, e, out_f32, static_cast<float *>(segments), s);
-    return launch_recurrent(p, e, out_f32, s);
+// Runs the passes, those that one launch can hold together.
+static void launch_passes(const MixPass *passes, int n, Element e, cudaStream_t s) {
+    enum Kind { TENSOR, BLOCK, TOKENS };
+    Kind kind[kMostPasses];
+    int shape[kMostPasses];
+    for (int k = 0; k < n; k++) {
+        kind[k] = chunked_tc_takes(passes[k], e) ? TENSOR : chunked_tf32_takes(passes[k]) ? BLOCK : TOKENS;
+        shape[k] = kind[k] == TENSOR ? chunked_tc_shape(passes[k]) : kind[k] == BLOCK ? chunked_tf32_shape(passes[k]) : 0;
+    }
+    bool gone[kMostPasses] = {};
+    for (int k = 0; k < n; k++) {
+        if (gone[k]) continue;
+        MixPass together[kMostPasses];
+        int m = 0;
+        for (int j = k; j < n; j++)
+            if (!gone[j] && kind[j] == kind[k] && shape[j] == shape[k] && (m == 0 || passes[k].p.batch * (m + 1) <= 65535) &&
+                (m == 0 || kind[k] != TOKENS)) {
+                together[m++] = passes[j];
+                gone[j] = true;
+            }
+        check(kind[k] == TENSOR  ? launch_chunked_tc(together, m, e, s)
+              : kind[k] == BLOCK ? launch_chunked_tf32(together, m, e, s)
+                                 : launch_recurrent(together[0], e, s),
+              "kernel launch");
+    }
 }
 
 static MixOperand operand(const void *p, const AttentionTensor &t, int per_head) { return {p, t.sb, t.st, t.sh, per_head}; }
 
-static MixParams common(const Context *ctx, const LinearAttention &a, const float *log_decay, const int64_t *offsets) {
-    MixParams p{};
+static MixPass common(const Context *ctx, const LinearAttention &a, const float *log_decay, const int64_t *offsets,
+                      int passes) {
+    MixPass pass{};
+    const Segments g = a.segments(passes);
+    pass.count = g.count;
+    pass.chunks = g.chunks;
+    MixParams &p = pass.p;
     p.log_decay = log_decay;
     p.offsets = offsets;
     p.length = a.length;
@@ -180,7 +212,7 @@ static MixParams common(const Context *ctx, const LinearAttention &a, const floa
     p.batch = a.batch;
     p.heads = (int)a.heads;
     p.err = ctx->d_err;
-    return p;
+    return pass;
 }
 
 static void output_to(MixParams &p, void *o, const AttentionTensor &t) {
@@ -208,7 +240,9 @@ void execute_linear_attention(Context *ctx, const LinearAttention &a, const b200
     std::lock_guard<std::mutex> l(ctx->mu);
     if (!stream) stream = ctx->stream;
     if (!workspace && a.workspace()) workspace = context_scratch(ctx, a.workspace());
-    MixParams p = common(ctx, a, b.log_decay, a.packed ? b.sequence_offsets : nullptr);
+    MixPass pass = common(ctx, a, b.log_decay, a.packed ? b.sequence_offsets : nullptr, 1);
+    pass.segments = static_cast<float *>(workspace);
+    MixParams &p = pass.p;
     p.q = operand(b.query, a.q, 1);
     p.k = operand(b.key, a.k, a.share());
     p.v = operand(b.value, a.v, a.share());
@@ -223,7 +257,7 @@ void execute_linear_attention(Context *ctx, const LinearAttention &a, const b200
     p.dv = (int)a.value_dim;
     p.update = 1.f;
     p.out = a.scale;
-    check(launch_mix(p, a.element, false, workspace, stream), "kernel launch");
+    launch_passes(&pass, 1, a.element, stream);
 }
 
 void execute_linear_attention_grad(Context *ctx, const LinearAttention &a,
@@ -248,69 +282,72 @@ void execute_linear_attention_grad(Context *ctx, const LinearAttention &a,
     if (!stream) stream = ctx->stream;
     const int share = a.share();
     if (!workspace && a.backward_workspace()) workspace = context_scratch(ctx, a.backward_workspace());
-    const MixParams base = common(ctx, a, g.log_decay, a.packed ? g.sequence_offsets : nullptr);
+    const MixPass base = common(ctx, a, g.log_decay, a.packed ? g.sequence_offsets : nullptr, kMostPasses);
     const MixOperand q = operand(g.query, a.q, 1), k = operand(g.key, a.k, share), v = operand(g.value, a.v, share),
                      d = operand(g.output_gradient, a.o, 1);
-
-    if (g.query_gradient) {  // dq = scale * the operator on (do, v, k), from the transposed initial state
-        MixParams p = base;
-        p.q = d, p.k = v, p.v = k;
-        output_to(p, g.query_gradient, a.q);
-        p.s_in = g.initial_state;
-        p.state_slots = a.batch;
-        p.state_k = 1;
-        p.state_v = a.value_dim;
-        p.dk = (int)a.value_dim;
-        p.dv = (int)a.key_dim;
-        p.update = 1.f;
-        p.out = a.scale;
-        check(launch_mix(p, a.element, false, workspace, stream), "kernel launch");
-    }
-    // dk and dv run from the last token back; their state is the state's gradient
-    auto late = [&](const MixOperand &rq, const MixOperand &rk, const MixOperand &rv, int64_t dk, int64_t dv,
-                    int64_t state_k, int64_t state_v, void *out, const AttentionTensor &t, float *partial, float *s_out) {
-        MixParams p = base;
-        p.reverse = 1;
+    unsigned char *space = static_cast<unsigned char *>(workspace);
+    float *const partial = reinterpret_cast<float *>(space + kMostPasses * a.segment_bytes(kMostPasses));
+    MixPass passes[kMostPasses];
+    int n = 0;
+    auto add = [&](const MixOperand &rq, const MixOperand &rk, const MixOperand &rv, int64_t dk, int64_t dv) -> MixPass & {
+        MixPass &pass = passes[n];
+        pass = base;
+        pass.segments = reinterpret_cast<float *>(space + n * a.segment_bytes(kMostPasses));
+        n++;
+        MixParams &p = pass.p;
         p.q = rq, p.k = rk, p.v = rv;
-        p.s_in = g.final_state_gradient;
-        p.s_out = s_out;
         p.state_slots = a.batch;
-        p.state_k = state_k;
-        p.state_v = state_v;
         p.dk = (int)dk;
         p.dv = (int)dv;
+        // a state is [key_dim, value_dim]; this pass's first dimension may be the values'
+        const bool turned = &rq != &k;
+        p.state_k = turned ? 1 : a.value_dim;
+        p.state_v = turned ? a.value_dim : 1;
+        return pass;
+    };
+    if (g.query_gradient) {  // dq = scale * the operator on (do, v, k), from the transposed initial state
+        MixParams &p = add(d, v, k, a.value_dim, a.key_dim).p;
+        output_to(p, g.query_gradient, a.q);
+        p.s_in = g.initial_state;
+        p.update = 1.f;
+        p.out = a.scale;
+    }
+    // dk and dv run from the last token back; their state is the state's gradient, which the latter leaves
+    ShareParams sums{};
+    int shared = 0;
+    auto late = [&](MixPass &pass, void *out, const AttentionTensor &t, float *part) {
+        MixParams &p = pass.p;
+        p.reverse = 1;
+        p.s_in = g.final_state_gradient;
         p.update = a.scale;
         p.out = 1.f;
         if (share == 1 || !out) {
             output_to(p, out, t);
-        } else {
-            const AttentionTensor dense{a.length * a.heads * dv, a.heads * dv, dv, dv};
-            output_to(p, partial, dense);
+            return;
         }
-        check(launch_mix(p, a.element, share > 1, workspace, stream), "kernel launch");
-        if (share > 1 && out) {
-            ShareParams sp{};
-            sp.src = partial;
-            sp.dst = out;
-            sp.sb = t.sb, sp.st = t.st, sp.sh = t.sh;
-            sp.offsets = base.offsets;
-            sp.length = a.length;
-            sp.packed_tokens = a.packed_tokens;
-            sp.batch = a.batch;
-            sp.kv_heads = (int)a.kv_heads;
-            sp.share = share;
-            sp.dim = (int)dv;
-            check(launch_share(sp, a.element, stream), "kernel launch");
-        }
+        const int64_t dim = t.dim;
+        output_to(p, part, AttentionTensor{a.length * a.heads * dim, a.heads * dim, dim, dim});
+        pass.out_f32 = 1;
+        sums.tensor[shared++] = ShareTensor{part, out, t.sb, t.st, t.sh, (int)dim};
     };
-    float *part_k = reinterpret_cast<float *>(static_cast<unsigned char *>(workspace) + a.segment_bytes()), *part_v = part_k + (share > 1 ? a.tokens() * a.heads * a.key_dim : 0);
-    // the state's own gradient comes out of the last pass that reads the final state's, which it may replace
-    if (g.key_gradient)
-        late(v, d, q, a.value_dim, a.key_dim, 1, a.value_dim, g.key_gradient, a.k, part_k,
-             g.value_gradient ? nullptr : g.initial_state_gradient);
-    if (g.value_gradient || (g.initial_state_gradient && !g.key_gradient)) {
-        void *out = g.value_gradient;
-        late(k, q, d, a.key_dim, a.value_dim, a.value_dim, 1, out, a.v, part_v, g.initial_state_gradient);
+    if (g.key_gradient) late(add(v, d, q, a.value_dim, a.key_dim), g.key_gradient, a.k, partial);
+    if (g.value_gradient || g.initial_state_gradient) {
+        MixPass &pass = add(k, q, d, a.key_dim, a.value_dim);
+        late(pass, g.value_gradient, a.v, partial + a.tokens() * a.heads * a.key_dim);
+        pass.p.s_out = g.initial_state_gradient;
+    }
+    // where the state's gradient replaces the final state's, its pass runs after the one that also reads that
+    const bool after = g.key_gradient && g.initial_state_gradient && g.initial_state_gradient == g.final_state_gradient;
+    launch_passes(passes, after ? n - 1 : n, a.element, stream);
+    if (after) launch_passes(passes + n - 1, 1, a.element, stream);
+    if (shared) {
+        sums.offsets = base.p.offsets;
+        sums.length = a.length;
+        sums.packed_tokens = a.packed_tokens;
+        sums.batch = a.batch;
+        sums.kv_heads = (int)a.kv_heads;
+        sums.share = share;
+        check(launch_share(sums, shared, a.element, stream), "kernel launch");
     }
 }
 

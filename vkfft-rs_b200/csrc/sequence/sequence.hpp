@@ -56,6 +56,11 @@ cudaError_t launch_norm_grad(const NormGradParams &p, Element e, Element param, 
 
 // ---- linear attention -----------------------------------------------------------------
 
+struct Segments {
+    int count;   // of the longest sequence
+    int chunks;  // of 128 tokens, of each segment
+};
+
 struct AttentionTensor {
     int64_t sb, st, sh;  // elements between batches, tokens, heads
     int64_t dim;
@@ -70,8 +75,9 @@ struct LinearAttention {
     static LinearAttention from_c(const b200fft_linear_attention_config &c);
     int64_t tokens() const { return packed ? packed_tokens : batch * length; }
     int share() const { return static_cast<int>(heads / kv_heads); }
-    size_t segment_bytes() const;  // states between the segments of the sequences
-    size_t workspace() const { return segment_bytes(); }
+    Segments segments(int passes) const;
+    size_t segment_bytes(int passes) const;  // states between the segments of one of so many passes
+    size_t workspace() const { return segment_bytes(1); }
     size_t backward_workspace() const;
 };
 
@@ -106,34 +112,45 @@ struct MixParams {
     int *err;
 };
 
-// out_f32: o holds f32 whatever the element type (partial gradients of shared heads)
-cudaError_t launch_recurrent(const MixParams &p, Element e, bool out_f32, cudaStream_t s);
-
-// By chunks of tokens on the tensor cores; segments of a sequence run side by side, with a
-// pass before them that sums up each segment's own state (`segments`: batch x heads x
-// count x dk x dv floats where count > 1).
-struct Segments {
-    int count;   // of the longest sequence
-    int chunks;  // of each segment
+// One run of the recurrence: the forward pass is one, the gradients are three.
+struct MixPass {
+    MixParams p;
+    int out_f32;      // o holds f32 whatever the element type (partial gradients of shared heads)
+    // segments of each sequence that run side by side, after a pass that sums up each segment's own state
+    int count;        // of the longest sequence
+    int chunks;       // of 128 tokens, of each segment
+    float *segments;  // count > 1: [batch][heads][count][dk][dv], the segments' sums, then the states that enter them
 };
-Segments segments_of(int64_t length, int64_t batch, int64_t heads);
-bool chunked_tc_takes(const MixParams &p, Element e, bool out_f32);
-cudaError_t launch_chunked_tc(const MixParams &p, Element e, bool out_f32, float *segments, cudaStream_t s);
+constexpr int kMostPasses = 3;
 
+Segments segments_of(int64_t length, int64_t lines);
+
+// Token by token.
+cudaError_t launch_recurrent(const MixPass &pass, Element e, cudaStream_t s);
+// By chunks of tokens on the tensor cores (tcgen05): 16-bit types, 16-byte rows.  Passes of one shape (equal `shape`)
+// may go in one launch.
+bool chunked_tc_takes(const MixPass &pass, Element e);
+int chunked_tc_shape(const MixPass &pass);
+cudaError_t launch_chunked_tc(const MixPass *passes, int n, Element e, cudaStream_t s);
 // The same for every type, dimension, stride and address, on tf32 matrix instructions.
-bool chunked_tf32_takes(const MixParams &p);
-cudaError_t launch_chunked_tf32(const MixParams &p, Element e, bool out_f32, float *segments, cudaStream_t s);
+bool chunked_tf32_takes(const MixPass &pass);
+int chunked_tf32_shape(const MixPass &pass);
+cudaError_t launch_chunked_tf32(const MixPass *passes, int n, Element e, cudaStream_t s);
 
-// dst[.., g, d] = sum over the share query heads of src[token, g * share + j, d]
-struct ShareParams {
+// dst[.., g, d] = sum over the share query heads of src[token, g * share + j, d], for up to two tensors
+struct ShareTensor {
     const float *src;  // [tokens][kv_heads * share][dim], token as in the workspace
     void *dst;
     int64_t sb, st, sh;
+    int dim;
+};
+struct ShareParams {
+    ShareTensor tensor[2];
     const int64_t *offsets;
     int64_t length, packed_tokens, batch;
-    int kv_heads, share, dim;
+    int kv_heads, share;
 };
-cudaError_t launch_share(const ShareParams &p, Element e, cudaStream_t s);
+cudaError_t launch_share(const ShareParams &p, int tensors, Element e, cudaStream_t s);
 
 void execute_layer_norm(Context *ctx, const LayerNorm &n, const NormParams &p, cudaStream_t stream);
 void execute_layer_norm_grad(Context *ctx, const LayerNorm &n, NormGradParams p, void *workspace, cudaStream_t stream);
