@@ -10,7 +10,7 @@
 //   scores  [Q K^T]            128 x 128, decayed, rounded to bf16 in tensor memory (P)
 //   inside  [P V]              128 x dv
 //   before  [Q S]              128 x dv, S rounded to bf16 in shared memory; rows decayed in f32
-//   update  [W^T V]            dk x dv, W_j = l^(127-j) k_j as four bf16 terms that hold the 24
+//   update  [W^T V]            dk x dv, W_j = l^(127-j) k_j as bf16 terms that hold the 24
 //                              bits of the f32 product: the state is an f32 result and stays one
 // The two roundings (P, S) and the result's own are each half a unit of bf16: the result is
 // within sqrt(3) of the rounding that any bf16 result has.
@@ -197,9 +197,11 @@ __device__ __noinline__ void careful_rows(const unsigned char *sq, const unsigne
 
 // W of 16 tile rows and 32 key columns: the weights w = w1 + w2 + w3 (terms of the type) of this thread's rows,
 // 2 (lane % 4), 2 (lane % 4) + 1 and those 8 further on, times the keys.  k w1 = a + b and k w2 = c + d exactly (a
-// product of two mantissas is its rounding and a remainder of the type), so W = a + b + c + (d + k w3): only the last
-// sum is rounded, at 2^-25 of W in bf16.  Two terms are a and b + k w2, off by 2^-17 (f16: 2^-23).  Packed 16-bit
-// arithmetic: five (three) instructions for two rows; terms cut out of the f32 product took twice as many.  ldmatrix
+// product of two mantissas is its rounding and a remainder of the type), b + c = m + r exactly (the rounding of a sum and
+// what it left out), so W = a + m + (r + d + k w3): only the last is rounded, at 2^-25 of W in bf16.  As four terms it is
+// a, b, c and (d + k w3): fewer instructions (measured better where the warps have more to do), more products (which
+// bound the sum of a segment).  Two terms are a and b + k w2, off by 2^-17 (f16: 2^-23).  Packed 16-bit arithmetic; the
+// terms cut out of the f32 product took more.  ldmatrix
 // turns the keys the way the tensor memory wants them (a lane for each key column): one 2-byte load for each key had
 // bound this step.
 template <typename T, int TERMS>
@@ -221,9 +223,16 @@ __device__ __forceinline__ void make_weights(uint32_t keys, uint32_t unit, uint3
                 t[1][e] = as_word(__hfma2(k, w2, b));
             } else {
                 const P c = __hmul2_rn(k, w2), d = __hfma2(k, w2, __hneg2(c));
-                t[1][e] = as_word(b);
-                t[2][e] = as_word(c);
-                t[3][e] = as_word(__hfma2(k, as_two<T>(w[2][e >> 1]), d));
+                if (TERMS == 4) {
+                    t[1][e] = as_word(b);
+                    t[2][e] = as_word(c);
+                    t[TERMS - 1][e] = as_word(__hfma2(k, as_two<T>(w[2][e >> 1]), d));
+                    continue;
+                }
+                const P m = __hadd2_rn(b, c), c0 = __hsub2_rn(m, b), b0 = __hsub2_rn(m, c0);
+                const P r = __hadd2_rn(__hsub2_rn(b, b0), __hsub2_rn(c, c0));
+                t[1][e] = as_word(m);
+                t[2][e] = as_word(__hadd2_rn(r, __hfma2(k, as_two<T>(w[2][e >> 1]), d)));
             }
         }
 #pragma unroll
@@ -274,16 +283,16 @@ __device__ __forceinline__ void clear_rows(unsigned char *tiles, int first, int 
     compute_sync();
 }
 
-// A segment's own sum: what its tokens leave of the state at its end, from a state of zero.  Four terms, as it is an
+// A segment's own sum: what its tokens leave of the state at its end, from a state of zero.  Three terms, as it is an
 // f32 result; and the chunks add up in registers, one chunk behind the products: the tensor cores cut sums off where
 // f32 rounds, which over a whole segment would be 2 to 4e-6 of the result, to one side.
-template <typename T, int DK, int DV>
+template <typename T, int DK, int DV, bool MANY>
 __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant__ TensorPasses run) {
     using L = SumLayout<DK, DV>;
     constexpr int COLS = DV / kGroups;
     constexpr bool HALF = std::is_same<T, __half>::value;
-    constexpr int TERMS = HALF ? 2 : 4;
-    constexpr int kBuffers = HALF ? 3 : 2;              // of W for half a chunk
+    constexpr int TERMS = HALF ? 2 : 3;
+    constexpr int kBuffers = HALF ? 3 : 2;              // of W for half a chunk: what 256 columns hold
     constexpr uint32_t kWColumns = TERMS * 32, kSums = 256;  // W buffers from column 0; the products of two chunks in turn
     extern __shared__ unsigned char raw[];
     __shared__ __align__(8) uint64_t bars[3 * L::stages + 2 * kBuffers + 2];
@@ -292,7 +301,8 @@ __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant_
     __shared__ float pw[kChunk + 1];  // l^n, times `update` or f16's weight factor
     __shared__ uint32_t key_most[2][L::stages];
 
-    const int pass = blockIdx.z / (unsigned)run.all.pass[0].p.batch, b = blockIdx.z % (unsigned)run.all.pass[0].p.batch;
+    const int pass = MANY ? blockIdx.z / (unsigned)run.all.pass[0].p.batch : 0;
+    const int b = MANY ? blockIdx.z % (unsigned)run.all.pass[0].p.batch : blockIdx.z;
     const MixPass &cp = run.all.pass[pass];
     const Maps &maps = run.maps[pass];
     const MixParams &p = cp.p;
@@ -334,6 +344,8 @@ __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant_
         float s[COLS];
 #pragma unroll
         for (int j = 0; j < COLS; j++) s[j] = 0.f;
+        int weights_of = 0;
+        uint32_t w[2][3][2];
         Scale before{1.f, 1.f};
         const Fade whole = fade_of((double)log_decay * kChunk);
         // reverse: the decay of a row itself; f16 multiplies by it here, as its weights would underflow together
@@ -361,26 +373,30 @@ __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant_
                 key = key_scale_of(max(key_most[0][stage], key_most[1][stage]));
             }
             const uint32_t key_factor = HALF ? pack<T>(key.up, key.up) : 0;
+            if (n != weights_of) {  // the first chunk, and a last one that is shorter
+                weights_of = n;
+#pragma unroll
+                for (int half = 0; half < 2; half++)
+#pragma unroll
+                    for (int pair = 0; pair < 2; pair++) {
+                        float f[2];
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const int r = half * 64 + group * 16 + 2 * (lane & 3) + 8 * pair + e;
+                            f[e] = r >= first && r < end ? pw[p.reverse ? r + OWN - first : end - 1 - r] : 0.f;
+                        }
+                        split_terms<T, TERMS == 2 ? 2 : 3>(f[0], f[1], &w[half][0][pair], 2);
+                    }
+            }
 #pragma unroll
             for (int half = 0; half < 2; half++) {
-                const int i = 2 * c + half, buffer = i % kBuffers, r0 = half * 64 + group * 16 + 2 * (lane & 3);
-                uint32_t w[3][2];
-#pragma unroll
-                for (int pair = 0; pair < 2; pair++) {
-                    float f[2];
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const int r = r0 + 8 * pair + e;
-                        f[e] = r >= first && r < end ? pw[p.reverse ? r + OWN - first : end - 1 - r] : 0.f;
-                    }
-                    split_terms<T, TERMS == 2 ? 2 : 3>(f[0], f[1], &w[0][pair], 2);
-                }
+                const int i = 2 * c + half, buffer = i % kBuffers;
                 if (i >= kBuffers) {
                     barrier_wait(used + 8 * buffer, (i / kBuffers - 1) & 1, gone);
                     fence_after_sync();
                 }
                 if (row < DK)
-                    make_weights<T, TERMS>(keys + stage * L::stage + (half * 4 + group) * 2048, unit, key_factor, w,
+                    make_weights<T, TERMS>(keys + stage * L::stage + (half * 4 + group) * 2048, unit, key_factor, w[half],
                                     lanes + buffer * kWColumns + group * 8, 32);
                 tmem_store_wait();
                 fence_before_sync();
@@ -472,14 +488,16 @@ __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant_
 // The results of a segment, and (FINAL, one segment) the final state.
 // bf16 terms of the state update's weights: two (2^-17) where the state only goes on into results; four where it is
 // itself a result, in f32: then the weights of half a chunk fill the tensor memory that is left.
-template <typename T, int DK, int DV, bool FINAL>
+// MANY: several passes in one launch (their parameters are indexed, which costs registers).
+template <typename T, int DK, int DV, bool FINAL, bool MANY>
 __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constant__ TensorPasses run) {
     using L = Layout<DK, DV>;
     constexpr int COLS = DV / kGroups;  // state and result columns of one thread
     constexpr bool HALF = std::is_same<T, __half>::value;
     constexpr int TERMS = FINAL && !HALF ? 4 : 2, HALVES = TERMS == 4 ? 2 : 1, kTermColumns = kChunk / 2 / HALVES;
     extern __shared__ unsigned char raw[];
-    const int pass = blockIdx.z / (unsigned)run.all.pass[0].p.batch, b = blockIdx.z % (unsigned)run.all.pass[0].p.batch;
+    const int pass = MANY ? blockIdx.z / (unsigned)run.all.pass[0].p.batch : 0;
+    const int b = MANY ? blockIdx.z % (unsigned)run.all.pass[0].p.batch : blockIdx.z;
     const MixPass &cp = run.all.pass[pass];
     const Maps &maps = run.maps[pass];
     const MixParams &p = cp.p;
@@ -1108,25 +1126,25 @@ bool loadable(const MixOperand &t, int dim) {
            t.sh % 8 == 0 && t.sb < widest && t.st < widest && t.sh < widest;
 }
 
-template <typename T, int DK, int DV>
+template <typename T, int DK, int DV, bool MANY>
 cudaError_t launch_dims(const TensorPasses &run, int passes, cudaStream_t s) {
     const MixPass &first = run.all.pass[0];
     const dim3 grid(first.count, first.p.heads, (unsigned)first.p.batch * passes);
     if (first.count == 1)  // the state itself is a result (and, wanted or not, it makes the same results)
-        return launch(chunk_kernel<T, DK, DV, true>, grid, kThreads, shared_bytes(Layout<DK, DV>::bytes, sizeof(ChunkSmall)), false, s, run);
-    cudaError_t e = launch(sum_kernel<T, DK, DV>, grid, kThreads, shared_bytes(SumLayout<DK, DV>::bytes, 0), false, s, run);
+        return launch(chunk_kernel<T, DK, DV, true, MANY>, grid, kThreads, shared_bytes(Layout<DK, DV>::bytes, sizeof(ChunkSmall)), false, s, run);
+    cudaError_t e = launch(sum_kernel<T, DK, DV, MANY>, grid, kThreads, shared_bytes(SumLayout<DK, DV>::bytes, 0), false, s, run);
     if (e == cudaSuccess) e = launch_enter(run.all, passes, s);
     if (e != cudaSuccess) return e;
-    return launch(chunk_kernel<T, DK, DV, false>, grid, kThreads, shared_bytes(Layout<DK, DV>::bytes, sizeof(ChunkSmall)), true, s, run);
+    return launch(chunk_kernel<T, DK, DV, false, MANY>, grid, kThreads, shared_bytes(Layout<DK, DV>::bytes, sizeof(ChunkSmall)), true, s, run);
 }
 
-template <typename T>
+template <typename T, bool MANY>
 cudaError_t launch_type(const TensorPasses &run, int passes, cudaStream_t s) {
     switch (chunked_tc_shape(run.all.pass[0])) {
-        case 0: return launch_dims<T, 64, 64>(run, passes, s);
-        case 1: return launch_dims<T, 64, 128>(run, passes, s);
-        case 2: return launch_dims<T, 128, 64>(run, passes, s);
-        default: return launch_dims<T, 128, 128>(run, passes, s);
+        case 0: return launch_dims<T, 64, 64, MANY>(run, passes, s);
+        case 1: return launch_dims<T, 64, 128, MANY>(run, passes, s);
+        case 2: return launch_dims<T, 128, 64, MANY>(run, passes, s);
+        default: return launch_dims<T, 128, 128, MANY>(run, passes, s);
     }
 }
 
@@ -1172,7 +1190,8 @@ cudaError_t launch_chunked_tc(const MixPass *passes, int n, Element e, cudaStrea
         encode(run.maps[k].v, p.v, p, p.dv, e);
         if (p.o) encode(run.maps[k].o, {p.o, p.osb, p.ost, p.osh, 1}, p, p.dv, passes[k].out_f32 ? Element::F32 : e);
     }
-    return e == Element::F16 ? launch_type<__half>(run, n, s) : launch_type<__nv_bfloat16>(run, n, s);
+    if (e == Element::F16) return n > 1 ? launch_type<__half, true>(run, n, s) : launch_type<__half, false>(run, n, s);
+    return n > 1 ? launch_type<__nv_bfloat16, true>(run, n, s) : launch_type<__nv_bfloat16, false>(run, n, s);
 }
 
 }  // namespace b200fft
