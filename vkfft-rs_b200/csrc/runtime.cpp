@@ -335,7 +335,7 @@ void execute_program_host(Context *ctx, uint64_t id, const Program &prog, const 
 static std::string describe_error_word(int err) {
     std::string m = "B200 FFT kernel reported error word " + std::to_string(err);
     if (err & 32) m += " (slab exchange barrier timed out: a peer rank did not arrive)";
-    if (err & 64) m += " (linear attention: a wait for the tensor cores or a copy expired)";
+    if (err & 64) m += " (a wait for the tensor cores or for a copy expired)";
     if (err & ~(32 | 64)) m += " (invalid pass program)";
     return m;
 }

@@ -26,6 +26,34 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
+// Two f32 at once.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void split_pair(uint64_t p, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// One f32, where a kernel is written for either.
+__device__ __forceinline__ float mul_pair(float a, float b) { return a * b; }
+__device__ __forceinline__ float add_pair(float a, float b) { return a + b; }
+__device__ __forceinline__ float fma_pair(float a, float b, float c) { return fmaf(a, b, c); }
+
 // First row and number of rows of sequence b.  Offsets are data: whatever they hold, the
 // range stays inside the packed rows and no longer than `length`.
 struct Rows {

@@ -2,6 +2,7 @@
 #include <algorithm>
 
 #include "launch.cuh"
+#include "tcgen05.cuh"
 
 namespace b200fft {
 
@@ -28,50 +29,76 @@ __device__ __forceinline__ float block_sum(float v, float *buf) {
 // rows or addresses are not aligned): one read, mean and centred variance from registers, one write.  Bound by HBM;
 // the weight and bias come from L1 after the first row.
 
-template <typename T, int VEC>
-struct Vec {
-    float f[VEC];
-    __device__ __forceinline__ void load(const T *p) {
-        if constexpr (VEC == 1) {
-            f[0] = to_float(*p);
-        } else {
-            static_assert(VEC * sizeof(T) == 16, "16 bytes");
-            const uint4 w = *reinterpret_cast<const uint4 *>(p);
-            const T *e = reinterpret_cast<const T *>(&w);
-#pragma unroll
-            for (int i = 0; i < VEC; i++) f[i] = to_float(e[i]);
-        }
-    }
-    __device__ __forceinline__ void store(T *p) const {
-        if constexpr (VEC == 1) {
-            *p = from_float<T>(f[0]);
-        } else {
-            uint4 w;
-            T *e = reinterpret_cast<T *>(&w);
-#pragma unroll
-            for (int i = 0; i < VEC; i++) e[i] = from_float<T>(f[i]);
-            *reinterpret_cast<uint4 *>(p) = w;
-        }
-    }
-};
-
+// Rows go by once: loads and stores that do not stay in the caches (16384 x 4096 bf16: 54 -> 52 us).
 // The raw 16 bytes (or one element) of a vector, as they wait for their turn.
 template <typename T, int VEC>
 struct Raw {
     uint4 w;
-    __device__ __forceinline__ void load(const T *p) { w = *reinterpret_cast<const uint4 *>(p); }
-    __device__ __forceinline__ float at(int i) const { return to_float(reinterpret_cast<const T *>(&w)[i]); }
+    __device__ __forceinline__ void load(const T *p) { w = __ldcs(reinterpret_cast<const uint4 *>(p)); }
+    __device__ __forceinline__ void load_shared(const T *p) { w = *reinterpret_cast<const uint4 *>(p); }
+    __device__ __forceinline__ uint32_t word(int k) const { return k == 0 ? w.x : k == 1 ? w.y : k == 2 ? w.z : w.w; }
+    // elements 2 i and 2 i + 1
+    __device__ __forceinline__ uint64_t pair(int i) const {
+        if constexpr (std::is_same<T, float>::value) {
+            return pair_of(__uint_as_float(word(2 * i)), __uint_as_float(word(2 * i + 1)));
+        } else if constexpr (std::is_same<T, __half>::value) {
+            const uint32_t v = word(i);
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&v));
+            return pair_of(f.x, f.y);
+        } else {
+            return pair_of(__uint_as_float(word(i) << 16), __uint_as_float(word(i) & 0xffff0000u));
+        }
+    }
 };
 template <typename T>
 struct Raw<T, 1> {
     T w;
     __device__ __forceinline__ void load(const T *p) { w = *p; }
-    __device__ __forceinline__ float at(int) const { return to_float(w); }
+    __device__ __forceinline__ float pair(int) const { return to_float(w); }
+};
+// VEC elements as pairs of f32, of which one instruction does both; a single element by itself.
+template <int VEC>
+using Lane = typename std::conditional<VEC == 1, float, uint64_t>::type;
+template <typename L>
+__device__ __forceinline__ L both(float v) {
+    if constexpr (std::is_same<L, float>::value)
+        return v;
+    else
+        return pair_of(v, v);
+}
+__device__ __forceinline__ void take(uint64_t p, float *f) { split_pair(p, f[0], f[1]); }
+__device__ __forceinline__ void take(float p, float *f) { f[0] = p; }
+__device__ __forceinline__ float sum_of(float p) { return p; }
+__device__ __forceinline__ float sum_of(uint64_t p) {
+    float a, b;
+    split_pair(p, a, b);
+    return a + b;
+}
+template <int VEC>
+struct Pairs {
+    static constexpr int N = (VEC + 1) / 2;
+    Lane<VEC> p[N];
+    template <typename T>
+    __device__ __forceinline__ void store(T *to) const {
+        float f[2 * N];
+#pragma unroll
+        for (int i = 0; i < N; i++) take(p[i], f + 2 * i);
+        if constexpr (VEC == 1) {
+            *to = from_float<T>(f[0]);
+        } else {
+            uint4 w;
+            T *e = reinterpret_cast<T *>(&w);
+#pragma unroll
+            for (int i = 0; i < VEC; i++) e[i] = from_float<T>(f[i]);
+            __stcs(reinterpret_cast<uint4 *>(to), w);
+        }
+    }
 };
 
 // VEC parameters of whatever type, from an index that is a multiple of VEC; aligned where VEC > 1.
 template <int VEC>
-__device__ __forceinline__ void load_parameters(const void *p, Element type, int64_t at, float (&f)[VEC]) {
+__device__ __forceinline__ void load_parameters(const void *p, Element type, int64_t at, Pairs<VEC> &to) {
+    float f[2 * Pairs<VEC>::N] = {};
     if (type == Element::F32) {
         const float *q = static_cast<const float *>(p) + at;
         if constexpr (VEC == 1) {
@@ -100,6 +127,13 @@ __device__ __forceinline__ void load_parameters(const void *p, Element type, int
             const uint16_t bits = (uint16_t)(w[i / 2] >> (i % 2 * 16));
             f[i] = type == Element::F16 ? __half2float(__ushort_as_half(bits)) : __uint_as_float((uint32_t)bits << 16);
         }
+    }
+#pragma unroll
+    for (int i = 0; i < Pairs<VEC>::N; i++) {
+        if constexpr (VEC == 1)
+            to.p[i] = f[0];
+        else
+            to.p[i] = pair_of(f[2 * i], f[2 * i + 1]);
     }
 }
 
@@ -136,43 +170,56 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_kernel(const __gri
     const T *x = static_cast<const T *>(p.x) + row * p.xs;
     T *y = static_cast<T *>(p.y) + row * p.ys;
     const int units = (int)p.features / VEC;
-    Vec<T, VEC> v[VPT];
-    float s[1] = {0.f};
+    constexpr int N = Pairs<VEC>::N;
+    Pairs<VEC> v[VPT];
+    {
+        Raw<T, VEC> raw[VPT];
 #pragma unroll
-    for (int k = 0; k < VPT; k++)
-        if (at + k * TPR < units) v[k].load(x + (at + k * TPR) * VEC);
+        for (int k = 0; k < VPT; k++)
+            if (at + k * TPR < units) raw[k].load(x + (at + k * TPR) * VEC);
+#pragma unroll
+        for (int k = 0; k < VPT; k++)
+#pragma unroll
+            for (int i = 0; i < N; i++) v[k].p[i] = raw[k].pair(i);
+    }
+    Lane<VEC> sum = both<Lane<VEC>>(0.f);
 #pragma unroll
     for (int k = 0; k < VPT; k++)
         if (at + k * TPR < units) {
 #pragma unroll
-            for (int i = 0; i < VEC; i++) s[0] += v[k].f[i];
+            for (int i = 0; i < N; i++) sum = add_pair(sum, v[k].p[i]);
         }
+    float s[1] = {sum_of(sum)};
     row_sums<TPR>(s, buf[0]);
     const float mean = s[0] / (float)p.features;
-    s[0] = 0.f;
+    sum = both<Lane<VEC>>(0.f);
 #pragma unroll
     for (int k = 0; k < VPT; k++)
         if (at + k * TPR < units) {
 #pragma unroll
-            for (int i = 0; i < VEC; i++) {
-                v[k].f[i] -= mean;
-                s[0] = fmaf(v[k].f[i], v[k].f[i], s[0]);
+            for (int i = 0; i < N; i++) {
+                v[k].p[i] = add_pair(v[k].p[i], both<Lane<VEC>>(-mean));
+                sum = fma_pair(v[k].p[i], v[k].p[i], sum);
             }
         }
+    s[0] = sum_of(sum);
     row_sums<TPR>(s, buf[1]);
     const float rstd = 1.f / sqrtf(s[0] / (float)p.features + p.epsilon);
 #pragma unroll
     for (int k = 0; k < VPT; k++)
         if (at + k * TPR < units) {
-            float w[VEC], b[VEC];
-            if (p.w) load_parameters<VEC>(p.w, p.parameter, (at + k * TPR) * VEC, w);
-            if (p.b) load_parameters<VEC>(p.b, p.parameter, (at + k * TPR) * VEC, b);
 #pragma unroll
-            for (int i = 0; i < VEC; i++) {
-                float f = v[k].f[i] * rstd;
-                if (p.w) f *= w[i];
-                if (p.b) f += b[i];
-                v[k].f[i] = f;
+            for (int i = 0; i < N; i++) v[k].p[i] = mul_pair(v[k].p[i], both<Lane<VEC>>(rstd));
+            Pairs<VEC> w;
+            if (p.w) {
+                load_parameters<VEC>(p.w, p.parameter, (at + k * TPR) * VEC, w);
+#pragma unroll
+                for (int i = 0; i < N; i++) v[k].p[i] = mul_pair(v[k].p[i], w.p[i]);
+            }
+            if (p.b) {
+                load_parameters<VEC>(p.b, p.parameter, (at + k * TPR) * VEC, w);
+#pragma unroll
+                for (int i = 0; i < N; i++) v[k].p[i] = add_pair(v[k].p[i], w.p[i]);
             }
             v[k].store(y + (at + k * TPR) * VEC);
         }
@@ -187,7 +234,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_kernel(const __gri
 // sums in registers.  Otherwise (rows of 1024 threads, whose 64 registers do not hold that) they stand in shared memory:
 // 8 bytes read and written for each element, half of what the row takes from HBM at HBM's pace.
 template <typename T, int VEC, int TPR, int VPT, bool NEXT>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR <= 256 ? 2 : 1) norm_grad_kernel(const __grid_constant__ NormGradParams p) {
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, VEC == 1 ? 1024 / (TPR < 256 ? 256 : TPR) : TPR <= 256 ? 2 : 1) norm_grad_kernel(const __grid_constant__ NormGradParams p) {
     constexpr int BLOCK = TPR < 256 ? 256 : TPR, GROUPS = BLOCK / TPR;
     __shared__ float buf[2][BLOCK / 32 * 2];
     extern __shared__ __align__(16) float columns[];  // [2][VPT][VEC][TPR]
@@ -195,7 +242,8 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR <= 256 ? 2 : 1) nor
     const int64_t group = (int64_t)blockIdx.x * GROUPS + threadIdx.x / TPR;
     const int units = (int)p.features / VEC;
     const float scale = 1.f / (float)p.features;
-    float w[VPT][VEC], dw[NEXT ? VPT : 1][VEC], db[NEXT ? VPT : 1][VEC];
+    constexpr int N = Pairs<VEC>::N;
+    Pairs<VEC> w[VPT], dw[NEXT ? VPT : 1], db[NEXT ? VPT : 1];
     Raw<T, VEC> x[VPT], dy[VPT];
     float mean = 0.f, rstd = 0.f;
     auto fetch = [&](int64_t row) {
@@ -214,12 +262,13 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR <= 256 ? 2 : 1) nor
 #pragma unroll
     for (int k = 0; k < VPT; k++) {
 #pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            w[k][i] = 1.f;
-            if constexpr (NEXT)
-                dw[k][i] = db[k][i] = 0.f;
-            else
-                columns[(k * VEC + i) * TPR + at] = columns[((VPT + k) * VEC + i) * TPR + at] = 0.f;
+        for (int i = 0; i < N; i++) {
+            w[k].p[i] = both<Lane<VEC>>(1.f);
+            if constexpr (NEXT) dw[k].p[i] = db[k].p[i] = both<Lane<VEC>>(0.f);
+        }
+        if constexpr (!NEXT) {
+#pragma unroll
+            for (int i = 0; i < VEC; i++) columns[(k * VEC + i) * TPR + at] = columns[((VPT + k) * VEC + i) * TPR + at] = 0.f;
         }
         if (p.w && at + k * TPR < units) load_parameters<VEC>(p.w, p.parameter, (at + k * TPR) * VEC, w[k]);
     }
@@ -230,28 +279,36 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR <= 256 ? 2 : 1) nor
         const bool live = row < p.rows && group < p.partials;
         const float m = mean, r = rstd;
         Raw<T, VEC> x0[VPT], dy0[VPT];
-        float s[2] = {0.f, 0.f};
+        Lane<VEC> s0 = both<Lane<VEC>>(0.f), s1 = both<Lane<VEC>>(0.f);
 #pragma unroll
         for (int k = 0; k < VPT; k++) {
             x0[k] = x[k];
             dy0[k] = dy[k];
             if (live && at + k * TPR < units) {
 #pragma unroll
-                for (int i = 0; i < VEC; i++) {
-                    const float d = dy0[k].at(i), h = (x0[k].at(i) - m) * r, g = d * w[k][i];
+                for (int i = 0; i < N; i++) {
+                    const Lane<VEC> d = dy0[k].pair(i), h = mul_pair(add_pair(x0[k].pair(i), both<Lane<VEC>>(-m)), both<Lane<VEC>>(r));
                     if constexpr (NEXT) {
-                        dw[k][i] = fmaf(d, h, dw[k][i]);
-                        db[k][i] += d;
+                        dw[k].p[i] = fma_pair(d, h, dw[k].p[i]);
+                        db[k].p[i] = add_pair(db[k].p[i], d);
                     } else {
-                        float &cw = columns[(k * VEC + i) * TPR + at], &cb = columns[((VPT + k) * VEC + i) * TPR + at];
-                        cw = fmaf(d, h, cw);
-                        cb += d;
+                        float d2[2], h2[2];
+                        take(d, d2);
+                        take(h, h2);
+#pragma unroll
+                        for (int e = 0; e < (VEC == 1 ? 1 : 2); e++) {
+                            float &cw = columns[(k * VEC + 2 * i + e) * TPR + at], &cb = columns[((VPT + k) * VEC + 2 * i + e) * TPR + at];
+                            cw = fmaf(d2[e], h2[e], cw);
+                            cb += d2[e];
+                        }
                     }
-                    s[0] += g;
-                    s[1] = fmaf(g, h, s[1]);
+                    const Lane<VEC> g = mul_pair(d, w[k].p[i]);
+                    s0 = add_pair(s0, g);
+                    s1 = fma_pair(g, h, s1);
                 }
             }
         }
+        float s[2] = {sum_of(s0), sum_of(s1)};
         if (NEXT) fetch(row + p.partials);
         row_sums<TPR>(s, buf[step & 1]);
         if (live && p.dx) {
@@ -260,11 +317,12 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR <= 256 ? 2 : 1) nor
 #pragma unroll
             for (int k = 0; k < VPT; k++)
                 if (at + k * TPR < units) {
-                    Vec<T, VEC> o;
+                    Pairs<VEC> o;
 #pragma unroll
-                    for (int i = 0; i < VEC; i++) {
-                        const float h = (x0[k].at(i) - m) * r, g = dy0[k].at(i) * w[k][i];
-                        o.f[i] = r * (g - a - h * b);
+                    for (int i = 0; i < N; i++) {
+                        const Lane<VEC> h = mul_pair(add_pair(x0[k].pair(i), both<Lane<VEC>>(-m)), both<Lane<VEC>>(r));
+                        const Lane<VEC> g = fma_pair(dy0[k].pair(i), w[k].p[i], both<Lane<VEC>>(-a));
+                        o.p[i] = mul_pair(fma_pair(h, both<Lane<VEC>>(-b), g), both<Lane<VEC>>(r));
                     }
                     o.store(dx + (at + k * TPR) * VEC);
                 }
@@ -277,11 +335,19 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR <= 256 ? 2 : 1) nor
     for (int k = 0; k < VPT; k++)
         if (at + k * TPR < units) {
             const int64_t to = group * p.features + (at + k * TPR) * VEC;
-            float a[VEC], b[VEC];
+            float a[2 * N], b[2 * N];
+            if constexpr (NEXT) {
 #pragma unroll
-            for (int i = 0; i < VEC; i++) {
-                a[i] = NEXT ? dw[NEXT ? k : 0][i] : columns[(k * VEC + i) * TPR + at];
-                b[i] = NEXT ? db[NEXT ? k : 0][i] : columns[((VPT + k) * VEC + i) * TPR + at];
+                for (int i = 0; i < N; i++) {
+                    take(dw[k].p[i], a + 2 * i);
+                    take(db[k].p[i], b + 2 * i);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; i++) {
+                    a[i] = columns[(k * VEC + i) * TPR + at];
+                    b[i] = columns[((VPT + k) * VEC + i) * TPR + at];
+                }
             }
             if constexpr (VEC == 1) {
                 p.part_w[to] = a[0];
@@ -292,6 +358,112 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR <= 256 ? 2 : 1) nor
                     *reinterpret_cast<float4 *>(p.part_w + to + i) = make_float4(a[i], a[i + 1], a[i + 2], a[i + 3]);
                     *reinterpret_cast<float4 *>(p.part_b + to + i) = make_float4(b[i], b[i + 1], b[i + 2], b[i + 3]);
                 }
+            }
+        }
+}
+
+// The same with rows that come through a ring of shared memory: whole rows of x and dy as bulk copies, up to
+// 208 KB of them on their way to an SM, where registers held one row ahead (32 KB on an SM at 4096 columns of bf16;
+// HBM's latency takes 50 KB and more).  One group to a CTA, 512 threads to an SM.
+__host__ __device__ constexpr int ring_bytes(int threads) { return 208 * 1024 / 512 * threads; }
+template <typename T, int TPR, int VPT>
+__global__ void __launch_bounds__(TPR, 512 / TPR) norm_grad_ring_kernel(const __grid_constant__ NormGradParams p) {
+    constexpr int VEC = 16 / sizeof(T), MOST = 16;
+    __shared__ __align__(8) uint64_t full[MOST];
+    __shared__ float buf[2][TPR / 32 * 2];
+    __shared__ int dead;
+    extern __shared__ __align__(128) unsigned char ring[];
+    const int at = threadIdx.x, group = blockIdx.x;
+    const int units = (int)p.features / VEC, bytes = units * 16;
+    const int stages = min(MOST, ring_bytes(TPR) / (2 * bytes));
+    const int64_t steps = (p.rows - group + p.partials - 1) / p.partials;
+    const float scale = 1.f / (float)p.features;
+    const uint32_t bar0 = shared_address(full), ring0 = shared_address(ring);
+    if (at == 0) {
+        for (int k = 0; k < stages; k++) barrier_init(bar0 + 8 * k, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        dead = 0;
+    }
+    __syncthreads();
+    auto fetch = [&](int64_t step, int stage) {  // by one thread
+        const int64_t row = group + step * p.partials;
+        const uint32_t bar = bar0 + 8 * stage, dst = ring0 + stage * 2 * bytes;
+        barrier_expect(bar, 2 * bytes);
+        bulk_load(dst, static_cast<const T *>(p.x) + row * p.xs, bytes, bar);
+        bulk_load(dst + bytes, static_cast<const T *>(p.dy) + row * p.ys, bytes, bar);
+    };
+    if (at == 0)
+        for (int k = 0; k < stages && k < steps; k++) fetch(k, k);
+    constexpr int N = Pairs<VEC>::N;
+    Pairs<VEC> w[VPT], dw[VPT], db[VPT];
+#pragma unroll
+    for (int k = 0; k < VPT; k++) {
+#pragma unroll
+        for (int i = 0; i < N; i++) w[k].p[i] = both<Lane<VEC>>(1.f), dw[k].p[i] = db[k].p[i] = both<Lane<VEC>>(0.f);
+        if (p.w && at + k * TPR < units) load_parameters<VEC>(p.w, p.parameter, (at + k * TPR) * VEC, w[k]);
+    }
+    float mean = p.mean[group], rstd = p.rstd[group];
+    int stage = 0, parity = 0;
+    for (int64_t step = 0; step < steps; step++) {
+        const int64_t row = group + step * p.partials;
+        const float m = mean, r = rstd;
+        if (step + 1 < steps) mean = p.mean[row + p.partials], rstd = p.rstd[row + p.partials];
+        barrier_wait(bar0 + 8 * stage, parity, &dead);
+        Raw<T, VEC> x[VPT], dy[VPT];
+        const T *tile = reinterpret_cast<const T *>(ring + stage * 2 * bytes);
+        Lane<VEC> s0 = both<Lane<VEC>>(0.f), s1 = both<Lane<VEC>>(0.f);
+#pragma unroll
+        for (int k = 0; k < VPT; k++)
+            if (at + k * TPR < units) {
+                x[k].load_shared(tile + (at + k * TPR) * VEC);
+                dy[k].load_shared(tile + (units + at + k * TPR) * VEC);
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    const Lane<VEC> d = dy[k].pair(i), h = mul_pair(add_pair(x[k].pair(i), both<Lane<VEC>>(-m)), both<Lane<VEC>>(r));
+                    dw[k].p[i] = fma_pair(d, h, dw[k].p[i]);
+                    db[k].p[i] = add_pair(db[k].p[i], d);
+                    const Lane<VEC> g = mul_pair(d, w[k].p[i]);
+                    s0 = add_pair(s0, g);
+                    s1 = fma_pair(g, h, s1);
+                }
+            }
+        float s[2] = {sum_of(s0), sum_of(s1)};
+        row_sums<TPR>(s, buf[step & 1]);  // every thread has read its part of the stage
+        if (at == 0 && step + stages < steps && !dead) fetch(step + stages, stage);
+        if (++stage == stages) stage = 0, parity ^= 1;
+        if (p.dx) {
+            T *dx = static_cast<T *>(p.dx) + row * p.xs;
+            const float a = s[0] * scale, b = s[1] * scale;
+#pragma unroll
+            for (int k = 0; k < VPT; k++)
+                if (at + k * TPR < units) {
+                    Pairs<VEC> o;
+#pragma unroll
+                    for (int i = 0; i < N; i++) {
+                        const Lane<VEC> h = mul_pair(add_pair(x[k].pair(i), both<Lane<VEC>>(-m)), both<Lane<VEC>>(r));
+                        const Lane<VEC> g = fma_pair(dy[k].pair(i), w[k].p[i], both<Lane<VEC>>(-a));
+                        o.p[i] = mul_pair(fma_pair(h, both<Lane<VEC>>(-b), g), both<Lane<VEC>>(r));
+                    }
+                    o.store(dx + (at + k * TPR) * VEC);
+                }
+        }
+    }
+    let_next_start();
+    if (at == 0 && dead) {
+        atomicOr(p.err, 64);
+        for (int k = 0; k < stages; k++)  // copies that may still be on their way
+            for (int i = 0; i < 1 << 18 && !barrier_try(bar0 + 8 * k, k < stage ? parity ^ 1 : parity); i++) {
+            }
+    }
+    if (!p.part_w) return;
+#pragma unroll
+    for (int k = 0; k < VPT; k++)
+        if (at + k * TPR < units) {
+            const int64_t to = group * p.features + (at + k * TPR) * VEC;
+#pragma unroll
+            for (int i = 0; i < N; i += 2) {
+                *reinterpret_cast<ulonglong2 *>(p.part_w + to + 2 * i) = make_ulonglong2(dw[k].p[i], dw[k].p[i + 1]);
+                *reinterpret_cast<ulonglong2 *>(p.part_b + to + 2 * i) = make_ulonglong2(db[k].p[i], db[k].p[i + 1]);
             }
         }
 }
@@ -378,10 +550,12 @@ __global__ void __launch_bounds__(kThreads) norm_grad_columns_kernel(NormGradPar
     }
 }
 
-// Sums of the partials, in order: 32 columns x 8 lanes of partials, weight or bias by blockIdx.y.
+// Sums of the partials, in order: 32 columns x 32 lanes of partials, weight or bias by blockIdx.y.
+constexpr int kReduceThreads = 1024;
 template <typename P>
-__global__ void __launch_bounds__(kThreads) norm_grad_reduce_kernel(NormGradParams p) {
-    __shared__ float part[8][33];
+__global__ void __launch_bounds__(kReduceThreads) norm_grad_reduce_kernel(const __grid_constant__ NormGradParams p) {
+    constexpr int LANES = kReduceThreads / 32;
+    __shared__ float part[LANES][33];
     const int c = threadIdx.x & 31, lane = threadIdx.x >> 5;
     const int64_t col = (int64_t)blockIdx.x * 32 + c;
     const float *src = blockIdx.y ? p.part_b : p.part_w;
@@ -389,15 +563,15 @@ __global__ void __launch_bounds__(kThreads) norm_grad_reduce_kernel(NormGradPara
     wait_for_previous();
     float s = 0.f;
     if (dst && col < p.features) {
-#pragma unroll 8
-        for (int k = lane; k < p.partials; k += 8) s += src[k * p.features + col];
+#pragma unroll 16
+        for (int k = lane; k < p.partials; k += LANES) s += src[k * p.features + col];
     }
     part[lane][c] = s;
     __syncthreads();
-    if (lane == 0 && dst && col < p.features) {
-        for (int k = 1; k < 8; k++) s += part[k][c];
-        dst[col] = from_float<P>(s);
-    }
+    // the lanes of a column lie across the warps; warp c takes column c
+    s = warp_sum(part[c][lane]);
+    const int64_t mine = (int64_t)blockIdx.x * 32 + lane;
+    if (c == 0 && dst && mine < p.features) dst[mine] = from_float<P>(s);
 }
 
 int grid_of(int64_t n, int64_t most) { return (int)(n < most ? n : most); }
@@ -461,9 +635,9 @@ int norm_grad_groups(int64_t rows, int64_t features, int vec) {
                       : vec == 4 ? with_grad_shape<4>(features / 4, shape)
                                  : with_grad_shape<8>(features / 8, shape);
     if (!kept) return (int)std::clamp<int64_t>(rows / 64, 1, 64);
-    // as many rows at a time as fill the SMs with 512 threads each, but 8 rows or more to a group: its sums cost
-    // 8 bytes a column, written and read
-    const int64_t most = (int64_t)kSms * std::max(1, std::min(8, 512 / threads));
+    // as many rows at a time as fill the SMs (512 threads each, 1024 where a thread has four columns at most), but 8 rows
+    // or more to a group: its sums cost 8 bytes a column, written and read
+    const int64_t most = (int64_t)kSms * std::max(1, std::min(8, (vec == 1 ? 1024 : 512) / threads));
     return (int)std::clamp<int64_t>(rows / 8, 1, most);
 }
 
@@ -511,8 +685,11 @@ cudaError_t launch_norm_grad(const NormGradParams &args, Element e, Element para
             return with_grad_shape<V>(p.features / V, [&](auto tpr, auto vpt, auto next) {
                 constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value, GROUPS = TPR < 256 ? 256 / TPR : 1;
                 constexpr bool NEXT = decltype(next)::value;
-                started = launch(norm_grad_kernel<T, V, TPR, VPT, NEXT>, dim3((p.partials + GROUPS - 1) / GROUPS),
-                                 TPR < 256 ? 256 : TPR, NEXT ? 0 : 2 * VPT * V * TPR * (int)sizeof(float), false, s, p);
+                if constexpr (V > 1 && TPR >= 128 && NEXT)
+                    started = launch(norm_grad_ring_kernel<T, TPR, VPT>, dim3(p.partials), TPR, ring_bytes(TPR), false, s, p);
+                else
+                    started = launch(norm_grad_kernel<T, V, TPR, VPT, NEXT>, dim3((p.partials + GROUPS - 1) / GROUPS),
+                                     TPR < 256 ? 256 : TPR, NEXT ? 0 : 2 * VPT * V * TPR * (int)sizeof(float), false, s, p);
             });
         };
         return with_element(param, [&](auto q) {
@@ -530,7 +707,7 @@ cudaError_t launch_norm_grad(const NormGradParams &args, Element e, Element para
             }
             cudaError_t err = started != cudaSuccess ? started : cudaGetLastError();
             if (err == cudaSuccess && sums)
-                err = launch(norm_grad_reduce_kernel<P>, dim3((unsigned)((p.features + 31) / 32), 2), kThreads, 0, true, s, p);
+                err = launch(norm_grad_reduce_kernel<P>, dim3((unsigned)((p.features + 31) / 32), 2), kReduceThreads, 0, true, s, p);
             return err;
         });
     });

@@ -99,6 +99,7 @@ void execute_layer_norm_grad(Context *ctx, const LayerNorm &n, NormGradParams p,
     std::lock_guard<std::mutex> l(ctx->mu);
     if (!workspace && (p.dw || p.db)) workspace = context_scratch(ctx, n.backward_workspace());
     p.part_w = p.dw || p.db ? static_cast<float *>(workspace) : nullptr;
+    p.err = ctx->d_err;
     check(launch_norm_grad(p, n.element, n.parameter, stream ? stream : ctx->stream), "kernel launch");
 }
 

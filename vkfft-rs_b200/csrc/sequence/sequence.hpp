@@ -47,6 +47,7 @@ struct NormGradParams {
     int64_t features;
     int partials;
     Element parameter;
+    int *err;
 };
 // Groups of rows of the backward pass, for accesses of `vec` elements.
 int norm_grad_groups(int64_t rows, int64_t features, int vec);
