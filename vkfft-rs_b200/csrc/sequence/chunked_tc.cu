@@ -308,8 +308,9 @@ __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant_
     const MixParams &p = cp.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int segment = blockIdx.x, h = blockIdx.y;
-    const Line line(cp, segment, h, b);
+    wait_for_previous();
     let_next_start();
+    const Line line(cp, segment, h, b);
     if (segment > line.last || (segment == line.last && !p.s_out) || line.count == 0) return;
     const int chunks = (line.tokens + kChunk - 1) / kChunk;
 
@@ -503,7 +504,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     const MixParams &p = cp.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int segment = blockIdx.x, h = blockIdx.y;
+    if (FINAL) wait_for_previous();  // (otherwise the sum before has waited for the inputs)
     const Line line(cp, segment, h, b);
+    if (segment > line.last || line.count == 0) wait_for_previous();
     if (segment > line.last) return;
     const int chunks = (line.tokens + kChunk - 1) / kChunk;
     if (line.count == 0) {  // an empty sequence: its state passes through (with segments: before this kernel)
@@ -611,7 +614,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
             fence_async_shared();
         };
         {
-            wait_for_previous();
+            if (!FINAL) wait_for_previous();
+            let_next_start();
             const float *in = cp.count > 1 ? segment_state(cp, b, h, segment) : p.s_in && line.kept ? p.s_in + line.user : nullptr;
             const int64_t in_k = cp.count > 1 ? p.dv : p.state_k, in_v = cp.count > 1 ? 1 : p.state_v;
             const bool wide = in && in_v == 1 && (p.dv & 3) == 0 && (reinterpret_cast<uintptr_t>(in) & 15) == 0;
@@ -1131,11 +1135,11 @@ cudaError_t launch_dims(const TensorPasses &run, int passes, cudaStream_t s) {
     const MixPass &first = run.all.pass[0];
     const dim3 grid(first.count, first.p.heads, (unsigned)first.p.batch * passes);
     if (first.count == 1)  // the state itself is a result (and, wanted or not, it makes the same results)
-        return launch(chunk_kernel<T, DK, DV, true, MANY>, grid, kThreads, shared_bytes(Layout<DK, DV>::bytes, sizeof(ChunkSmall)), false, s, run);
-    cudaError_t e = launch(sum_kernel<T, DK, DV, MANY>, grid, kThreads, shared_bytes(SumLayout<DK, DV>::bytes, 0), false, s, run);
+        return launch(chunk_kernel<T, DK, DV, true, MANY>, grid, kThreads, shared_bytes(Layout<DK, DV>::bytes, sizeof(ChunkSmall)), s, run);
+    cudaError_t e = launch(sum_kernel<T, DK, DV, MANY>, grid, kThreads, shared_bytes(SumLayout<DK, DV>::bytes, 0), s, run);
     if (e == cudaSuccess) e = launch_enter(run.all, passes, s);
     if (e != cudaSuccess) return e;
-    return launch(chunk_kernel<T, DK, DV, false, MANY>, grid, kThreads, shared_bytes(Layout<DK, DV>::bytes, sizeof(ChunkSmall)), true, s, run);
+    return launch(chunk_kernel<T, DK, DV, false, MANY>, grid, kThreads, shared_bytes(Layout<DK, DV>::bytes, sizeof(ChunkSmall)), s, run);
 }
 
 template <typename T, bool MANY>

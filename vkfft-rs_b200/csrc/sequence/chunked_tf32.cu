@@ -126,10 +126,13 @@ __global__ void __launch_bounds__(kThreads) block_kernel(const __grid_constant__
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int slices = gridDim.y / p.heads;
     const int segment = blockIdx.x, h = blockIdx.y / slices, c0 = blockIdx.y % slices * kSlice;
-    if (c0 >= p.dv) return;  // the widest pass decides the grid
     const int cols = min(kSlice, p.dv - c0);
+    // (the pass after a sum: that has waited for the inputs)
+    if (SUM || cp.count == 1) wait_for_previous();
     const Line line(cp, segment, h, b);
+    if (!SUM && (segment > line.last || c0 >= p.dv)) wait_for_previous();
     if (SUM) let_next_start();
+    if (c0 >= p.dv) return;  // the widest pass decides the grid
     if (segment > line.last || (SUM && ((segment == line.last && !p.s_out) || line.count == 0))) return;
     const int chunks = (line.tokens + C - 1) / C;  // none for an empty sequence, whose state passes through
     const float log_decay = p.log_decay[h];
@@ -139,7 +142,8 @@ __global__ void __launch_bounds__(kThreads) block_kernel(const __grid_constant__
     const int state_row = warp / STATE_ACROSS * 16 * STATE_ROWS, state_col = warp % STATE_ACROSS * STATE_TILES * 8;
     float s[STATE_ROWS][STATE_TILES][4];
     float *const own = segment_state(cp, b, h, segment);
-    if (!SUM) wait_for_previous();
+    if (!SUM && cp.count > 1) wait_for_previous();
+    if (!SUM) let_next_start();
     const float *in = SUM ? nullptr : cp.count > 1 ? own : p.s_in && line.kept ? p.s_in + line.user : nullptr;
     float *out = SUM ? own : cp.count == 1 && p.s_out && line.kept ? p.s_out + line.user : nullptr;
     const int64_t in_k = cp.count > 1 ? p.dv : p.state_k, in_v = cp.count > 1 ? 1 : p.state_v;  // of `out` too
@@ -348,11 +352,11 @@ cudaError_t launch_dims(const Passes &all, int passes, cudaStream_t s) {
     for (int k = 0; k < passes; k++) slices = std::max(slices, (all.pass[k].p.dv + kSlice - 1) / kSlice);
     const dim3 grid(first.count, first.p.heads * slices, (unsigned)first.p.batch * passes);
     if (first.count > 1) {
-        cudaError_t e = launch(block_kernel<T, DK, true>, grid, kThreads, BlockLayout<DK>::bytes, false, s, all);
+        cudaError_t e = launch(block_kernel<T, DK, true>, grid, kThreads, BlockLayout<DK>::bytes, s, all);
         if (e == cudaSuccess) e = launch_enter(all, passes, s);
         if (e != cudaSuccess) return e;
     }
-    return launch(block_kernel<T, DK, false>, grid, kThreads, BlockLayout<DK>::bytes, first.count > 1, s, all);
+    return launch(block_kernel<T, DK, false>, grid, kThreads, BlockLayout<DK>::bytes, s, all);
 }
 
 }  // namespace

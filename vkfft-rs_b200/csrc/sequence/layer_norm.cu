@@ -166,10 +166,15 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_kernel(const __gri
     __shared__ float buf[2][BLOCK / 32];
     const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
     const int at = threadIdx.x % TPR;
-    if (TPR == 32 && row >= p.rows) return;  // (wider rows: a block is one row)
+    if (TPR == 32 && row >= p.rows) {  // (wider rows: a block is one row)
+        wait_for_previous();
+        return;
+    }
     const T *x = static_cast<const T *>(p.x) + row * p.xs;
     T *y = static_cast<T *>(p.y) + row * p.ys;
     const int units = (int)p.features / VEC;
+    wait_for_previous();
+    let_next_start();
     constexpr int N = Pairs<VEC>::N;
     Pairs<VEC> v[VPT];
     {
@@ -258,6 +263,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, VEC == 1 ? 1024 / (TPR 
         mean = p.mean[row];
         rstd = p.rstd[row];
     };
+    wait_for_previous();
     fetch(group);
 #pragma unroll
     for (int k = 0; k < VPT; k++) {
@@ -385,6 +391,7 @@ __global__ void __launch_bounds__(TPR, 512 / TPR) norm_grad_ring_kernel(const __
         dead = 0;
     }
     __syncthreads();
+    wait_for_previous();
     auto fetch = [&](int64_t step, int stage) {  // by one thread
         const int64_t row = group + step * p.partials;
         const uint32_t bar = bar0 + 8 * stage, dst = ring0 + stage * 2 * bytes;
@@ -470,8 +477,10 @@ __global__ void __launch_bounds__(TPR, 512 / TPR) norm_grad_ring_kernel(const __
 
 // A row of any width: one CTA reads it three times (the second and third from L1 or L2).
 template <typename T, typename P>
-__global__ void __launch_bounds__(kThreads) norm_long_kernel(NormParams p) {
+__global__ void __launch_bounds__(kThreads) norm_long_kernel(const __grid_constant__ NormParams p) {
     __shared__ float buf[kThreads / 32];
+    wait_for_previous();
+    let_next_start();
     const P *w = static_cast<const P *>(p.w), *b = static_cast<const P *>(p.b);
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const T *x = static_cast<const T *>(p.x) + row * p.xs;
@@ -499,8 +508,10 @@ __global__ void __launch_bounds__(kThreads) norm_long_kernel(NormParams p) {
 }
 
 template <typename T, typename P>
-__global__ void __launch_bounds__(kThreads) norm_grad_long_kernel(NormGradParams p) {
+__global__ void __launch_bounds__(kThreads) norm_grad_long_kernel(const __grid_constant__ NormGradParams p) {
     __shared__ float buf[kThreads / 32];
+    wait_for_previous();
+    let_next_start();
     const P *w = static_cast<const P *>(p.w);
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const T *x = static_cast<const T *>(p.x) + row * p.xs, *dy = static_cast<const T *>(p.dy) + row * p.ys;
@@ -524,8 +535,10 @@ __global__ void __launch_bounds__(kThreads) norm_grad_long_kernel(NormGradParams
 
 // Column sums of dy xhat and dy over one strip of rows: 32 columns x 8 row lanes.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) norm_grad_columns_kernel(NormGradParams p) {
+__global__ void __launch_bounds__(kThreads) norm_grad_columns_kernel(const __grid_constant__ NormGradParams p) {
     __shared__ float sw[8][33], sb[8][33];
+    wait_for_previous();
+    let_next_start();
     const int c = threadIdx.x & 31, lane = threadIdx.x >> 5;
     const int64_t col = (int64_t)blockIdx.x * 32 + c;
     const int64_t strip = (p.rows + p.partials - 1) / p.partials;
@@ -561,6 +574,7 @@ __global__ void __launch_bounds__(kReduceThreads) norm_grad_reduce_kernel(const 
     const float *src = blockIdx.y ? p.part_b : p.part_w;
     P *dst = static_cast<P *>(blockIdx.y ? p.db : p.dw);
     wait_for_previous();
+    let_next_start();
     float s = 0.f;
     if (dst && col < p.features) {
 #pragma unroll 16
@@ -647,24 +661,22 @@ cudaError_t launch_norm(const NormParams &args, Element e, Element param, cudaSt
     return with_element(e, [&](auto t) {
         using T = decltype(t);
         constexpr int VEC = 16 / sizeof(T);
+        cudaError_t started = cudaSuccess;
         const auto in_registers = [&](auto vec) {
             return with_row_shape(p.features / decltype(vec)::value, [&](auto tpr, auto vpt) {
                 constexpr int TPR = decltype(tpr)::value, ROWS = TPR < 128 ? 128 / TPR : 1;
-                before_launch();
-                norm_kernel<T, decltype(vec)::value, TPR, decltype(vpt)::value>
-                    <<<(unsigned)((p.rows + ROWS - 1) / ROWS), TPR < 128 ? 128 : TPR, 0, s>>>(p);
+                started = launch(norm_kernel<T, decltype(vec)::value, TPR, decltype(vpt)::value>,
+                                 dim3((unsigned)((p.rows + ROWS - 1) / ROWS)), TPR < 128 ? 128 : TPR, 0, s, p);
             });
         };
         const bool wide = p.features % VEC == 0 && aligned_rows<T>(p.x, p.xs) && aligned_rows<T>(p.y, p.ys) &&
                           aligned_rows<T>(p.w, 0) && aligned_rows<T>(p.b, 0);
         const bool few = p.rows < (int64_t(1) << 31);  // a launch's CTAs
         if (!few || !(wide ? in_registers(Int<VEC>()) : in_registers(Int<1>())))
-            with_element(param, [&](auto q) {
-                before_launch();
-                norm_long_kernel<T, decltype(q)><<<grid_of(p.rows, 1 << 30), kThreads, 0, s>>>(p);
-                return cudaSuccess;
+            return with_element(param, [&](auto q) {
+                return launch(norm_long_kernel<T, decltype(q)>, dim3(grid_of(p.rows, 1 << 30)), kThreads, 0, s, p);
             });
-        return cudaGetLastError();
+        return started;
     });
 }
 
@@ -686,28 +698,24 @@ cudaError_t launch_norm_grad(const NormGradParams &args, Element e, Element para
                 constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value, GROUPS = TPR < 256 ? 256 / TPR : 1;
                 constexpr bool NEXT = decltype(next)::value;
                 if constexpr (V > 1 && TPR >= 128 && NEXT)
-                    started = launch(norm_grad_ring_kernel<T, TPR, VPT>, dim3(p.partials), TPR, ring_bytes(TPR), false, s, p);
+                    started = launch(norm_grad_ring_kernel<T, TPR, VPT>, dim3(p.partials), TPR, ring_bytes(TPR), s, p);
                 else
                     started = launch(norm_grad_kernel<T, V, TPR, VPT, NEXT>, dim3((p.partials + GROUPS - 1) / GROUPS),
-                                     TPR < 256 ? 256 : TPR, NEXT ? 0 : 2 * VPT * V * TPR * (int)sizeof(float), false, s, p);
+                                     TPR < 256 ? 256 : TPR, NEXT ? 0 : 2 * VPT * V * TPR * (int)sizeof(float), s, p);
             });
         };
         return with_element(param, [&](auto q) {
             using P = decltype(q);
             if (!(wide ? in_registers(Int<VEC>()) : in_registers(Int<1>()))) {
                 // the sums first: dx may take the place of dy
-                if (sums) {
-                    before_launch();
-                    norm_grad_columns_kernel<T><<<dim3((unsigned)((p.features + 31) / 32), p.partials), kThreads, 0, s>>>(p);
-                }
-                if (p.dx) {
-                    before_launch();
-                    norm_grad_long_kernel<T, P><<<grid_of(p.rows, 1 << 30), kThreads, 0, s>>>(p);
-                }
+                if (sums)
+                    started = launch(norm_grad_columns_kernel<T>, dim3((unsigned)((p.features + 31) / 32), p.partials), kThreads, 0, s, p);
+                if (p.dx && started == cudaSuccess)
+                    started = launch(norm_grad_long_kernel<T, P>, dim3(grid_of(p.rows, 1 << 30)), kThreads, 0, s, p);
             }
-            cudaError_t err = started != cudaSuccess ? started : cudaGetLastError();
+            cudaError_t err = started;
             if (err == cudaSuccess && sums)
-                err = launch(norm_grad_reduce_kernel<P>, dim3((unsigned)((p.features + 31) / 32), 2), kReduceThreads, 0, true, s, p);
+                err = launch(norm_grad_reduce_kernel<P>, dim3((unsigned)((p.features + 31) / 32), 2), kReduceThreads, 0, s, p);
             return err;
         });
     });

@@ -1,7 +1,7 @@
 // The recurrence of linear attention, token by token: the form for single tokens.
 #include <algorithm>
 
-#include "device.cuh"
+#include "launch.cuh"
 
 namespace b200fft {
 
@@ -15,7 +15,7 @@ constexpr int kMaxDim = 256;
 // columns 4 lane .. 4 lane + 3 of rows group, group + 16, ..., so that a state's rows are
 // read and written in 128-byte runs.
 template <typename T, typename O, int ROWS>
-__global__ void __launch_bounds__(kThreads) recurrent_kernel(MixParams p) {
+__global__ void __launch_bounds__(kThreads) recurrent_kernel(const __grid_constant__ MixParams p) {
     __shared__ float sq[kMaxDim], sk[kMaxDim], sv[kSlice];
     __shared__ float so[kThreads / 32][kSlice];
     const int slices = (p.dv + kSlice - 1) / kSlice;
@@ -25,6 +25,8 @@ __global__ void __launch_bounds__(kThreads) recurrent_kernel(MixParams p) {
     const int64_t b = bh / p.heads;
     const int tid = threadIdx.x, lane = tid & 7, group = tid >> 3;
     const int c0 = slice * kSlice + lane * 4;
+    wait_for_previous();
+    let_next_start();
     const Rows rows = rows_of(p.offsets, p.packed_tokens, p.length, b);
 
     const int64_t slot = p.slots ? p.slots[b] : b;
@@ -108,16 +110,10 @@ __global__ void __launch_bounds__(kThreads) recurrent_kernel(MixParams p) {
 template <typename T, typename O>
 cudaError_t launch_typed(const MixParams &p, cudaStream_t s) {
     const unsigned grid = (unsigned)(p.batch * p.heads * ((p.dv + kSlice - 1) / kSlice));
-    before_launch();
-    if (p.dk <= 32)
-        recurrent_kernel<T, O, 2><<<grid, kThreads, 0, s>>>(p);
-    else if (p.dk <= 64)
-        recurrent_kernel<T, O, 4><<<grid, kThreads, 0, s>>>(p);
-    else if (p.dk <= 128)
-        recurrent_kernel<T, O, 8><<<grid, kThreads, 0, s>>>(p);
-    else
-        recurrent_kernel<T, O, 16><<<grid, kThreads, 0, s>>>(p);
-    return cudaGetLastError();
+    if (p.dk <= 32) return launch(recurrent_kernel<T, O, 2>, dim3(grid), kThreads, 0, s, p);
+    if (p.dk <= 64) return launch(recurrent_kernel<T, O, 4>, dim3(grid), kThreads, 0, s, p);
+    if (p.dk <= 128) return launch(recurrent_kernel<T, O, 8>, dim3(grid), kThreads, 0, s, p);
+    return launch(recurrent_kernel<T, O, 16>, dim3(grid), kThreads, 0, s, p);
 }
 
 // Sums the partial gradients of the query heads that share a key/value head, in head order: VEC dimensions to a
@@ -126,6 +122,8 @@ constexpr int kTokens = 8;
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) share_kernel(const __grid_constant__ ShareParams p) {
     const ShareTensor &t = p.tensor[blockIdx.z];
+    wait_for_previous();
+    let_next_start();
     const int64_t b = blockIdx.y;
     const Rows rows = rows_of(p.offsets, p.packed_tokens, p.length, b);
     const int64_t token0 = (int64_t)blockIdx.x * kTokens;
@@ -178,12 +176,7 @@ cudaError_t launch_share(const ShareParams &p, int tensors, Element e, cudaStrea
     return with_element(e, [&](auto v) {
         using T = decltype(v);
         const dim3 grid((unsigned)((p.length + kTokens - 1) / kTokens), (unsigned)p.batch, (unsigned)tensors);
-        before_launch();
-        if (four)
-            share_kernel<T, 4><<<grid, 256, 0, s>>>(p);
-        else
-            share_kernel<T, 1><<<grid, 256, 0, s>>>(p);
-        return cudaGetLastError();
+        return four ? launch(share_kernel<T, 4>, grid, 256, 0, s, p) : launch(share_kernel<T, 1>, grid, 256, 0, s, p);
     });
 }
 

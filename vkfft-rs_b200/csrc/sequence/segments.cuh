@@ -110,7 +110,7 @@ inline cudaError_t launch_enter(const Passes &all, int passes, cudaStream_t s) {
     for (int k = 0; k < passes; k++) four = four && all.pass[k].p.dv % 4 == 0;
     const int vec = four ? 4 : 1;
     const dim3 grid((p.dk * p.dv + 128 * vec - 1) / (128 * vec), p.heads, (unsigned)p.batch * passes);
-    return four ? launch(enter_kernel<4>, grid, 128, 0, true, s, all) : launch(enter_kernel<1>, grid, 128, 0, true, s, all);
+    return four ? launch(enter_kernel<4>, grid, 128, 0, s, all) : launch(enter_kernel<1>, grid, 128, 0, s, all);
 }
 
 }  // namespace

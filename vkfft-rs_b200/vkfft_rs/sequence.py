@@ -15,6 +15,12 @@ stream.  A pointer of 0 leaves an optional tensor out.
 import ctypes
 import enum
 
+try:
+    from . import _calls
+except ImportError as e:
+    raise ImportError("vkfft_rs/_calls.so is missing: build it with `make -C vkfft-rs_b200` "
+                      "or __graft_entry__.build()") from e
+
 u64 = ctypes.c_uint64
 i32 = ctypes.c_int32
 vp = ctypes.c_void_p
@@ -39,17 +45,6 @@ class _LinearAttention(ctypes.Structure):
                 ("output_strides", u64 * 3)]
 
 
-class _Buffers(ctypes.Structure):
-    _fields_ = [(n, vp) for n in ("query", "key", "value", "log_decay", "sequence_offsets", "state_slots",
-                                  "initial_state", "output", "final_state")]
-
-
-class _Gradients(ctypes.Structure):
-    _fields_ = [(n, vp) for n in ("query", "key", "value", "log_decay", "sequence_offsets", "initial_state",
-                                  "output_gradient", "final_state_gradient", "query_gradient", "key_gradient",
-                                  "value_gradient", "initial_state_gradient")]
-
-
 def signatures():
     P = ctypes.POINTER
     return {
@@ -66,8 +61,8 @@ def signatures():
         "b200fft_linear_attention_destroy": ([vp], None),
         "b200fft_linear_attention_workspace_bytes": ([vp], u64),
         "b200fft_linear_attention_backward_workspace_bytes": ([vp], u64),
-        "b200fft_execute_linear_attention": ([vp, vp, P(_Buffers), vp, vp], i32),
-        "b200fft_execute_linear_attention_backward": ([vp, vp, P(_Gradients), vp, vp], i32),
+        "b200fft_execute_linear_attention": ([vp] * 5, i32),
+        "b200fft_execute_linear_attention_backward": ([vp] * 5, i32),
     }
 
 
@@ -205,39 +200,57 @@ class LinearAttentionIr(_Ir):
         return int(_api().library().b200fft_linear_attention_workspace_bytes(self._h))
 
 
+_addresses = {}
+
+
+def _address(name):
+    """Address of a function of the C ABI, for _calls."""
+    found = _addresses.get(name)
+    if found is None:
+        found = _addresses[name] = ctypes.cast(getattr(_api().library(), name), vp).value
+    return found
+
+
 class SequenceExecution:
-    """The sequence operators of a CudaExecutionContext."""
+    """The sequence operators of a CudaExecutionContext.  Tensors are device addresses (integers)."""
 
     def execute_layer_norm(self, ir, input_ptr, output_ptr, weight_ptr=0, bias_ptr=0, mean_ptr=0, rstd_ptr=0, stream=0):
         """y = (x - mean) rstd weight + bias; mean and rstd (f32) are written where given."""
-        api = _api()
-        api._check(api._lib.b200fft_execute_layer_norm(self._h, ir._h, input_ptr, weight_ptr, bias_ptr, output_ptr,
-                                                       mean_ptr, rstd_ptr, stream))
+        status = _calls.call(_address("b200fft_execute_layer_norm"), self._h.value or 0, ir._h.value, input_ptr, weight_ptr,
+                             bias_ptr, output_ptr, mean_ptr, rstd_ptr, stream)
+        if status:
+            _api()._check(status)
 
     def execute_layer_norm_backward(self, ir, input_ptr, mean_ptr, rstd_ptr, output_gradient_ptr, weight_ptr=0,
                                     input_gradient_ptr=0, weight_gradient_ptr=0, bias_gradient_ptr=0,
                                     workspace_ptr=0, stream=0):
-        api = _api()
-        api._check(api._lib.b200fft_execute_layer_norm_backward(
-            self._h, ir._h, input_ptr, weight_ptr, mean_ptr, rstd_ptr, output_gradient_ptr, input_gradient_ptr,
-            weight_gradient_ptr, bias_gradient_ptr, workspace_ptr, stream))
+        status = _calls.call(_address("b200fft_execute_layer_norm_backward"), self._h.value or 0, ir._h.value, input_ptr,
+                             weight_ptr, mean_ptr, rstd_ptr, output_gradient_ptr, input_gradient_ptr,
+                             weight_gradient_ptr, bias_gradient_ptr, workspace_ptr, stream)
+        if status:
+            _api()._check(status)
 
     def execute_linear_attention(self, ir, query_ptr, key_ptr, value_ptr, log_decay_ptr, output_ptr,
                                  initial_state_ptr=0, final_state_ptr=0, sequence_offsets_ptr=0, state_slots_ptr=0,
                                  workspace_ptr=0, stream=0):
         """Whole sequences, or (length 1) one new token of each, from initial_state to final_state."""
-        api = _api()
-        b = _Buffers(query_ptr, key_ptr, value_ptr, log_decay_ptr, sequence_offsets_ptr, state_slots_ptr,
-                     initial_state_ptr, output_ptr, final_state_ptr)
-        api._check(api._lib.b200fft_execute_linear_attention(self._h, ir._h, b, workspace_ptr, stream))
+        # the fields of b200fft_linear_attention_buffers, in order
+        status = _calls.call_struct(_address("b200fft_execute_linear_attention"), self._h.value or 0, ir._h.value, workspace_ptr,
+                                    stream, query_ptr, key_ptr, value_ptr, log_decay_ptr, sequence_offsets_ptr,
+                                    state_slots_ptr, initial_state_ptr, output_ptr, final_state_ptr)
+        if status:
+            _api()._check(status)
 
     def execute_linear_attention_backward(self, ir, query_ptr, key_ptr, value_ptr, log_decay_ptr, output_gradient_ptr,
                                           query_gradient_ptr=0, key_gradient_ptr=0, value_gradient_ptr=0,
                                           initial_state_ptr=0, final_state_gradient_ptr=0,
                                           initial_state_gradient_ptr=0, sequence_offsets_ptr=0, workspace_ptr=0,
                                           stream=0):
-        api = _api()
-        g = _Gradients(query_ptr, key_ptr, value_ptr, log_decay_ptr, sequence_offsets_ptr, initial_state_ptr,
-                       output_gradient_ptr, final_state_gradient_ptr, query_gradient_ptr, key_gradient_ptr,
-                       value_gradient_ptr, initial_state_gradient_ptr)
-        api._check(api._lib.b200fft_execute_linear_attention_backward(self._h, ir._h, g, workspace_ptr, stream))
+        # the fields of b200fft_linear_attention_gradients, in order
+        status = _calls.call_struct(_address("b200fft_execute_linear_attention_backward"), self._h.value or 0, ir._h.value,
+                                    workspace_ptr, stream, query_ptr, key_ptr, value_ptr, log_decay_ptr,
+                                    sequence_offsets_ptr, initial_state_ptr, output_gradient_ptr,
+                                    final_state_gradient_ptr, query_gradient_ptr, key_gradient_ptr, value_gradient_ptr,
+                                    initial_state_gradient_ptr)
+        if status:
+            _api()._check(status)
