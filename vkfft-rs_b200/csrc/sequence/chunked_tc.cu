@@ -35,8 +35,7 @@ constexpr int kComputeRegisters = 104, kOtherRegisters = 64;
 static_assert(kComputeWarps * 32 * kComputeRegisters + 128 * kOtherRegisters <= kThreads * 96, "register shares");
 constexpr int kGroups = kComputeWarps / 4;  // each has all 128 tensor memory lanes and a share of the columns
 constexpr uint32_t kTmemColumns = 512;
-// tensor memory columns: scores and P; results; state update; W terms
-constexpr uint32_t kX = 0, kY = 128, kZ = 256, kW = 384;
+constexpr uint32_t kX = 0, kY = 128;  // tensor memory columns of the scores and P, and of the results
 constexpr int kPanel = kChunk * 128;  // bytes of 128 rows x 64 elements
 
 struct Maps {
@@ -488,14 +487,17 @@ __global__ void __launch_bounds__(kThreads, 1) sum_kernel(const __grid_constant_
 
 // The results of a segment, and (FINAL, one segment) the final state.
 // bf16 terms of the state update's weights: two (2^-17) where the state only goes on into results; four where it is
-// itself a result, in f32: then the weights of half a chunk fill the tensor memory that is left.
+// itself a result, in f32: then the weights of half a chunk fill the tensor memory that is left (64 value columns leave
+// room for all, which measured slower: 57 against 53 us for the packed prompts of 64).
 // MANY: several passes in one launch (their parameters are indexed, which costs registers).
 template <typename T, int DK, int DV, bool FINAL, bool MANY>
 __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constant__ TensorPasses run) {
     using L = Layout<DK, DV>;
     constexpr int COLS = DV / kGroups;  // state and result columns of one thread
     constexpr bool HALF = std::is_same<T, __half>::value;
-    constexpr int TERMS = FINAL && !HALF ? 4 : 2, HALVES = TERMS == 4 ? 2 : 1, kTermColumns = kChunk / 2 / HALVES;
+    constexpr int TERMS = FINAL && !HALF ? 4 : 2, HALVES = TERMS == 4 ? 2 : 1;
+    constexpr uint32_t kTermColumns = kChunk / 2 / HALVES, kZ = kY + DV, kW = kZ + DV;  // the state update, W's terms
+    static_assert(kW + TERMS * kTermColumns <= kTmemColumns, "tensor memory");
     extern __shared__ unsigned char raw[];
     const int pass = MANY ? blockIdx.z / (unsigned)run.all.pass[0].p.batch : 0;
     const int b = MANY ? blockIdx.z % (unsigned)run.all.pass[0].p.batch : blockIdx.z;
@@ -1130,10 +1132,25 @@ bool loadable(const MixOperand &t, int dim) {
            t.sh % 8 == 0 && t.sb < widest && t.st < widest && t.sh < widest;
 }
 
+// Warpgroups that ask for more registers than the CTA was launched with would wait for good: not launched then.
+template <typename Kernel>
+void check_registers(Kernel *kernel) {
+    cudaFuncAttributes a;
+    if (cudaFuncGetAttributes(&a, kernel) != cudaSuccess || a.numRegs < 96)
+        fail_runtime("linear attention kernel was built with fewer registers than its warps share out");
+}
+
 template <typename T, int DK, int DV, bool MANY>
 cudaError_t launch_dims(const TensorPasses &run, int passes, cudaStream_t s) {
     const MixPass &first = run.all.pass[0];
     const dim3 grid(first.count, first.p.heads, (unsigned)first.p.batch * passes);
+    static const bool checked = [] {
+        check_registers(chunk_kernel<T, DK, DV, true, MANY>);
+        check_registers(sum_kernel<T, DK, DV, MANY>);
+        check_registers(chunk_kernel<T, DK, DV, false, MANY>);
+        return true;
+    }();
+    (void)checked;
     if (first.count == 1)  // the state itself is a result (and, wanted or not, it makes the same results)
         return launch(chunk_kernel<T, DK, DV, true, MANY>, grid, kThreads, shared_bytes(Layout<DK, DV>::bytes, sizeof(ChunkSmall)), s, run);
     cudaError_t e = launch(sum_kernel<T, DK, DV, MANY>, grid, kThreads, shared_bytes(SumLayout<DK, DV>::bytes, 0), s, run);
