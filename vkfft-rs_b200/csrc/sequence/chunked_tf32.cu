@@ -30,12 +30,10 @@ struct BlockLayout {
     static constexpr int bytes = end * 4;
 };
 
-__device__ __forceinline__ uint32_t to_tf32(float x) {
-    uint32_t r;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-    return r;
-}
-// A fragment's elements: the upper 11 bits and, where the element has more, the next 11.
+// A fragment's elements: rounded to 11 bits, and what is left (of either sign), of which the instruction sees 11 bits:
+// 2^-22 of the element is lost, to either side.  (cvt.rna.tf32 for both parts made 15 instructions for each matrix
+// instruction, and 57 us of 2 x 1023 x 8 heads x 64 x 96 where this takes 48; cutting the first part off, too, one
+// instruction less, left 7e-7 of the result, to one side.)
 template <int N, bool WHOLE>
 struct Parts {
     uint32_t hi[N], lo[WHOLE ? 1 : N];
@@ -43,8 +41,8 @@ struct Parts {
         if (WHOLE) {
             hi[i] = __float_as_uint(x);
         } else {
-            hi[i] = to_tf32(x);
-            lo[i] = to_tf32(x - __uint_as_float(hi[i]));
+            hi[i] = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+            lo[i] = __float_as_uint(x - __uint_as_float(hi[i]));
         }
     }
 };
@@ -53,16 +51,34 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
-// The instruction cuts sums off where f32 rounds; so each eight products are added up by themselves, and to the rest in
-// f32 (added to it by the instruction, 128 of them were off by 2e-6, to one side).
+// c += the products of two steps of eight.  The instruction cuts sums off where f32 rounds; so those sixteen are added up
+// by themselves, and to the rest in f32 (added to it by the instruction, 128 of them were off by 2e-6, to one side).
 template <bool WA, bool WB>
-__device__ __forceinline__ void multiply(float (&c)[4], const Parts<4, WA> &a, const Parts<2, WB> &b) {
+__device__ __forceinline__ void multiply(float (&c)[4], const Parts<4, WA> (&a)[2], const Parts<2, WB> (&b)[2]) {
     float x[4] = {0.f, 0.f, 0.f, 0.f};
-    if constexpr (!WA) mma_tf32(x, a.lo, b.hi);
-    if constexpr (!WB) mma_tf32(x, a.hi, b.lo);
-    mma_tf32(x, a.hi, b.hi);
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        if constexpr (!WA) mma_tf32(x, a[k].lo, b[k].hi);
+        if constexpr (!WB) mma_tf32(x, a[k].hi, b[k].lo);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; k++) mma_tf32(x, a[k].hi, b[k].hi);
 #pragma unroll
     for (int i = 0; i < 4; i++) c[i] += x[i];
+}
+// Fragments of two steps: A's rows by lane / 4, its eight columns by lane % 4 (or, for B, rows and columns changed).
+template <bool W>
+__device__ __forceinline__ void fragment_a(Parts<4, W> (&a)[2], const float *p, int pitch) {
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        a[k].set(0, p[8 * k]), a[k].set(1, p[8 * k + 8 * pitch]);
+        a[k].set(2, p[8 * k + 4]), a[k].set(3, p[8 * k + 4 + 8 * pitch]);
+    }
+}
+template <bool W>
+__device__ __forceinline__ void fragment_b(Parts<2, W> (&b)[2], const float *p, int step) {  // `step` floats from k to k + 1
+#pragma unroll
+    for (int k = 0; k < 2; k++) b[k].set(0, p[8 * k * step]), b[k].set(1, p[(8 * k + 4) * step]);
 }
 
 // C rows x COLS columns into shared memory as f32; rows outside [first, end) and columns from `cols` on are zero.
@@ -207,16 +223,14 @@ __global__ void __launch_bounds__(kThreads) block_kernel(const __grid_constant__
             const int col0 = warp % ACROSS * SCORE_TILES * 8;
             const bool none = p.reverse ? col0 + SCORE_TILES * 8 <= row0 : col0 >= row0 + 16;
             if (!none) {
-#pragma unroll 4
-                for (int d = 0; d < DK; d += 8) {
-                    Parts<4, WHOLE> a;
-                    const float *qa = sq + (row0 + g) * L::key_pitch + d + t;
-                    a.set(0, qa[0]), a.set(1, qa[8 * L::key_pitch]), a.set(2, qa[4]), a.set(3, qa[8 * L::key_pitch + 4]);
+#pragma unroll 2
+                for (int d = 0; d < DK; d += 16) {
+                    Parts<4, WHOLE> a[2];
+                    fragment_a(a, sq + (row0 + g) * L::key_pitch + d + t, L::key_pitch);
 #pragma unroll
                     for (int m = 0; m < SCORE_TILES; m++) {
-                        Parts<2, WHOLE> w;
-                        const float *kb = sk + (col0 + 8 * m + g) * L::key_pitch + d + t;
-                        w.set(0, kb[0]), w.set(1, kb[4]);
+                        Parts<2, WHOLE> w[2];
+                        fragment_b(w, sk + (col0 + 8 * m + g) * L::key_pitch + d + t, 1);
                         multiply(x[m], a, w);
                     }
                 }
@@ -237,23 +251,28 @@ __global__ void __launch_bounds__(kThreads) block_kernel(const __grid_constant__
             for (int j = 0; j < STATE_TILES; j++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) s[m][j][e] = faded(s[m][j][e], keep);
-#pragma unroll 2
-        for (int r = 0; r < C; r += 8) {
-            const float w0 = weight[r + t], w1 = weight[r + t + 4];
-            Parts<4, false> a[STATE_ROWS];
+        if (state_col < cols) {
+#pragma unroll 1
+            for (int r = 0; r < C; r += 16) {
+                Parts<4, false> a[STATE_ROWS][2];
 #pragma unroll
-            for (int m = 0; m < STATE_ROWS; m++) {
-                const float *ka = sk + (r + t) * L::key_pitch + state_row + 16 * m + g;
-                a[m].set(0, ka[0] * w0), a[m].set(1, ka[8] * w0);
-                a[m].set(2, ka[4 * L::key_pitch] * w1), a[m].set(3, ka[4 * L::key_pitch + 8] * w1);
-            }
+                for (int k = 0; k < 2; k++) {
+                    const int r0 = r + 8 * k + t;
+                    const float w0 = weight[r0], w1 = weight[r0 + 4];
 #pragma unroll
-            for (int j = 0; j < STATE_TILES; j++) {
-                Parts<2, WHOLE> w;
-                const float *vb = sv + (r + t) * L::value_pitch + state_col + 8 * j + g;
-                w.set(0, vb[0]), w.set(1, vb[4 * L::value_pitch]);
+                    for (int m = 0; m < STATE_ROWS; m++) {
+                        const float *ka = sk + r0 * L::key_pitch + state_row + 16 * m + g;
+                        a[m][k].set(0, ka[0] * w0), a[m][k].set(1, ka[8] * w0);
+                        a[m][k].set(2, ka[4 * L::key_pitch] * w1), a[m][k].set(3, ka[4 * L::key_pitch + 8] * w1);
+                    }
+                }
 #pragma unroll
-                for (int m = 0; m < STATE_ROWS; m++) multiply(s[m][j], a[m], w);
+                for (int j = 0; j < STATE_TILES; j++) {
+                    Parts<2, WHOLE> w[2];
+                    fragment_b(w, sv + (r + t) * L::value_pitch + state_col + 8 * j + g, L::value_pitch);
+#pragma unroll
+                    for (int m = 0; m < STATE_ROWS; m++) multiply(s[m][j], a[m], w);
+                }
             }
         }
         if (SUM) continue;
@@ -290,16 +309,15 @@ __global__ void __launch_bounds__(kThreads) block_kernel(const __grid_constant__
         // results: the state's part, faded by row, and the part inside the chunk
         const int col0 = warp % ACROSS * OUT_TILES * 8;
         float y[OUT_TILES][4] = {};
-#pragma unroll 4
-        for (int d = 0; d < DK; d += 8) {
-            Parts<4, WHOLE> a;
-            const float *qa = sq + (row0 + g) * L::key_pitch + d + t;
-            a.set(0, qa[0]), a.set(1, qa[8 * L::key_pitch]), a.set(2, qa[4]), a.set(3, qa[8 * L::key_pitch + 4]);
+        if (col0 >= cols) continue;  // columns past the last
+#pragma unroll 2
+        for (int d = 0; d < DK; d += 16) {
+            Parts<4, WHOLE> a[2];
+            fragment_a(a, sq + (row0 + g) * L::key_pitch + d + t, L::key_pitch);
 #pragma unroll
             for (int m = 0; m < OUT_TILES; m++) {
-                Parts<2, false> w;
-                const float *sb = ss + (d + t) * L::value_pitch + col0 + 8 * m + g;
-                w.set(0, sb[0]), w.set(1, sb[4 * L::value_pitch]);
+                Parts<2, false> w[2];
+                fragment_b(w, ss + (d + t) * L::value_pitch + col0 + 8 * m + g, L::value_pitch);
                 multiply(y[m], a, w);
             }
         }
@@ -311,16 +329,14 @@ __global__ void __launch_bounds__(kThreads) block_kernel(const __grid_constant__
             for (int m = 0; m < OUT_TILES; m++) y[m][e] *= fade;
         }
         const int from = p.reverse ? row0 : 0, to = p.reverse ? C : row0 + 16;  // columns of scores that this row tile has
-#pragma unroll 2
-        for (int j = from; j < to; j += 8) {
-            Parts<4, false> a;
-            const float *pa = sp + (row0 + g) * L::score_pitch + j + t;
-            a.set(0, pa[0]), a.set(1, pa[8 * L::score_pitch]), a.set(2, pa[4]), a.set(3, pa[8 * L::score_pitch + 4]);
+#pragma unroll 1
+        for (int j = from; j < to; j += 16) {
+            Parts<4, false> a[2];
+            fragment_a(a, sp + (row0 + g) * L::score_pitch + j + t, L::score_pitch);
 #pragma unroll
             for (int m = 0; m < OUT_TILES; m++) {
-                Parts<2, WHOLE> w;
-                const float *vb = sv + (j + t) * L::value_pitch + col0 + 8 * m + g;
-                w.set(0, vb[0]), w.set(1, vb[4 * L::value_pitch]);
+                Parts<2, WHOLE> w[2];
+                fragment_b(w, sv + (j + t) * L::value_pitch + col0 + 8 * m + g, L::value_pitch);
                 multiply(y[m], a, w);
             }
         }
