@@ -1,0 +1,509 @@
+// Linear attention by chunks of tokens for everything that the tcgen05 kernels do not take: f32, head dimensions up to
+// 256 of any size, any strides and addresses.
+//
+// The same products as there, in f32 accuracy on bf16 matrix instructions: every operand is a sum of bf16 terms (three
+// for f32, two for f16 and one for bf16 inputs; three for what is computed), and of the products of terms those that
+// matter at 2^-24 are taken: a b = a0 b0 + a0 b1 + a1 b0 + a0 b2 + a1 b1 + a2 b0.  Each element is taken apart once, on
+// its way into shared memory, and read as whole fragments (ldmatrix): two instructions for each matrix instruction.
+// (On tf32 instructions, with each warp taking its fragments apart, it was six, and four times the time.)
+// A CTA takes up to 64 value columns of one segment of one head of one sequence; the part of the state that a warp
+// updates stays in its registers in f32, and the next chunk's elements come by cp.async while this one is worked on.
+// One CTA to an SM, as large as shared memory holds: with chunks of 32 tokens, two CTAs of 256 threads took 587 us of
+// 2 x 12960 x 8 heads x 64 x 64, where chunks of 64 take 217 (of which 33 is what memory needs).  Bound by instructions
+// around the products (1.9 a cycle; the matrix pipe is busy a third of the time): of 14000 cycles for a chunk of 64
+// tokens by 64 x 64 in f32, taking elements apart was 4100, scores 2800, the state's update 1600, results 4300; warps
+// with tiles of 16 x 32 in place of 16 x 16 (fewer reads, half as many warps) made it 15 % slower.
+#include <algorithm>
+
+#include "segments.cuh"
+#include "tcgen05.cuh"
+
+namespace b200fft {
+
+namespace {
+
+using bf16 = __nv_bfloat16;
+
+// Tiles in shared memory: planes of one term each, rows padded by 16 bytes so that eight of them fall on different banks.
+template <int ROWS, int COLS>
+struct Tile {
+    static constexpr int pitch = (COLS + 8) * 2, plane = ROWS * pitch;  // bytes
+};
+
+// SUM (below) has no more than the keys and the weighted values.
+template <typename T, int DK, bool SUM>
+struct BlockShape {
+    static constexpr int IN = std::is_same<T, float>::value ? 3 : std::is_same<T, __half>::value ? 2 : 1;  // terms of an input
+    static constexpr int C = DK == 256 ? 16 : DK == 128 ? 32 : 64;  // tokens of a chunk
+    static constexpr int SLICE = DK == 256 || DK == 32 ? 32 : 64;   // value columns of a CTA
+    static constexpr int THREADS = DK == 32 ? 256 : 512, WARPS = THREADS / 32;
+    using Keys = Tile<C, DK>;
+    using Values = Tile<C, SLICE>;
+    using Scores = Tile<C, C>;
+    using State = Tile<DK, SLICE>;
+    static constexpr int k = 0, w = k + IN * Keys::plane, pw = w + 3 * Values::plane, weight = pw + (C + 4) * 4,
+                         raw_k = weight + C * 4, raw_v = raw_k + C * DK * sizeof(T), raw_q = raw_v + C * SLICE * sizeof(T),
+                         q = raw_q + (SUM ? 0 : C * DK * sizeof(T)),
+                         v = q + IN * Keys::plane, p = v + IN * Values::plane, s = p + 3 * Scores::plane,
+                         bytes = SUM ? q : s + 3 * State::plane;
+    static_assert(bytes <= 227 * 1024 - 64, "shared memory");
+};
+
+template <bool FIRST>
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (FIRST)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool TRANSPOSED>
+__device__ __forceinline__ void load4(uint32_t at, uint32_t (&r)[4]) {
+    if constexpr (TRANSPOSED)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+template <bool TRANSPOSED>
+__device__ __forceinline__ void load2(uint32_t at, uint32_t (&r)[4]) {
+    if constexpr (TRANSPOSED)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(at) : "memory");
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(at) : "memory");
+}
+
+// An operand in shared memory for one warp: TERMS planes, and this lane's row for ldmatrix.
+// A (16 rows m, contiguous along k; ALONG: stored with m contiguous) and B (columns n; stored with k contiguous, or
+// ALONG n).
+struct Operand {
+    uint32_t at;
+    int pitch, plane;
+};
+template <bool ALONG>
+__device__ __forceinline__ Operand operand_a(uint32_t tile, int pitch, int plane, int m0) {
+    const int lane = threadIdx.x & 31, low = lane & 7, mid = lane >> 3 & 1, high = lane >> 4;
+    const int r = ALONG ? low + high * 8 : m0 + low + mid * 8, c = ALONG ? m0 + mid * 8 : high * 8;
+    return {tile + r * pitch + c * 2, pitch, plane};
+}
+template <bool ALONG>
+__device__ __forceinline__ Operand operand_b(uint32_t tile, int pitch, int plane, int n0) {
+    const int lane = threadIdx.x & 31, low = lane & 7, mid = lane >> 3 & 1, high = lane >> 4;
+    const int r = ALONG ? low + mid * 8 : n0 + low + high * 8, c = ALONG ? n0 + high * 8 : mid * 8;
+    return {tile + r * pitch + c * 2, pitch, plane};
+}
+
+// The products of terms i and sum - i, the smallest first.
+template <int TA, int TB, int SUM, int I, bool FIRST, int PAIR>
+__device__ __forceinline__ void product(float (&x)[2][4], const uint32_t (&a)[TA][4], const uint32_t (&b)[TB][4]) {
+    constexpr bool there = I < TA && SUM - I < TB;
+    if constexpr (there) {
+#pragma unroll
+        for (int e = 0; e < PAIR; e++) mma_bf16<FIRST>(x[e], a[I], b[SUM - I][2 * e], b[SUM - I][2 * e + 1]);
+    }
+    if constexpr (I < SUM)
+        product<TA, TB, SUM, I + 1, FIRST && !there, PAIR>(x, a, b);
+    else if constexpr (SUM > 0)
+        product<TA, TB, SUM - 1, 0, FIRST && !there, PAIR>(x, a, b);
+}
+
+// c += A B over steps [from, to) of 16.  The instruction cuts sums off where f32 rounds, so sixteen products (and their
+// terms, small ones first) are added up by themselves, and to the rest in f32.
+template <int TA, int TB, int N, bool A_ALONG, bool B_ALONG>
+__device__ __forceinline__ void multiply(float (&c)[N][4], const Operand &a, const Operand &b, int from, int to) {
+    constexpr int PAIR = N == 1 ? 1 : 2;
+#pragma unroll 1
+    for (int k = from; k < to; k++) {
+        uint32_t af[TA][4];
+#pragma unroll
+        for (int i = 0; i < TA; i++) load4<A_ALONG>(a.at + i * a.plane + k * (A_ALONG ? 16 * a.pitch : 32), af[i]);
+#pragma unroll
+        for (int n = 0; n < N; n += 2) {
+            uint32_t bf[TB][4];
+#pragma unroll
+            for (int j = 0; j < TB; j++) {
+                const uint32_t at = b.at + j * b.plane + k * (B_ALONG ? 16 * b.pitch : 32) + n / 2 * (B_ALONG ? 32 : 16 * b.pitch);
+                if (N == 1)
+                    load2<B_ALONG>(at, bf[j]);
+                else
+                    load4<B_ALONG>(at, bf[j]);
+            }
+            float x[2][4];
+            product<TA, TB, 2, 0, true, PAIR>(x, af, bf);
+#pragma unroll
+            for (int e = 0; e < PAIR; e++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) c[n + e][i] += x[e][i];
+        }
+    }
+}
+
+// The terms of two neighbours into their planes.
+template <int TERMS>
+__device__ __forceinline__ void put(unsigned char *at, int plane, float a, float b) {
+    uint32_t t[TERMS ? TERMS : 1];
+    split_terms<bf16, TERMS>(a, b, t, 1);
+#pragma unroll
+    for (int k = 0; k < TERMS; k++) *reinterpret_cast<uint32_t *>(at + k * plane) = t[k];
+}
+// Of four: eight bytes to a store, so that a warp's stores meet no bank twice.
+template <int TERMS>
+__device__ __forceinline__ void put4(unsigned char *at, int plane, float a, float b, float c, float d) {
+    uint2 t[TERMS ? TERMS : 1];
+    split_terms<bf16, TERMS>(a, b, &t[0].x, 2);
+    split_terms<bf16, TERMS>(c, d, &t[0].y, 2);
+#pragma unroll
+    for (int k = 0; k < TERMS; k++) *reinterpret_cast<uint2 *>(at + k * plane) = t[k];
+}
+template <int TERMS>
+__device__ __forceinline__ float get(const unsigned char *at, int plane) {
+    float f = 0.f;
+#pragma unroll
+    for (int k = TERMS - 1; k >= 0; k--) f += __bfloat162float(*reinterpret_cast<const bf16 *>(at + k * plane));
+    return f;
+}
+
+// there: otherwise nothing is read and zeros are written
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t to, const void *from, bool there) {
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? BYTES : 0) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES), "r"(there ? BYTES : 0) : "memory");
+}
+
+// C rows x COLS columns on their way into shared memory, four neighbours at a time; rows outside [first, end) and columns
+// from `cols` on are zero.  Each thread takes apart what it has fetched itself (convert), so the next chunk's elements
+// come while this one's are worked on, with no barrier between.
+template <typename T>
+struct __align__(sizeof(T) * 4) Piece {
+    T v[4];
+};
+template <typename T, int C, int COLS, int THREADS>
+__device__ __forceinline__ void fetch(unsigned char *raw, const T *src, int64_t stride, int first, int end, int cols) {
+    constexpr int ACROSS = COLS / 4, STEPS = (C * ACROSS + THREADS - 1) / THREADS;
+    static_assert(THREADS % ACROSS == 0, "a thread keeps its columns");
+    const bool wide = cols % 4 == 0 && stride % 4 == 0 && (reinterpret_cast<uintptr_t>(src) & (sizeof(Piece<T>) - 1)) == 0;
+    const int r0 = threadIdx.x / ACROSS, c = threadIdx.x % ACROSS * 4;
+    const uint32_t to = shared_address(raw) + threadIdx.x * sizeof(Piece<T>);
+    const T *safe = src + first * stride;  // an address to name where nothing is read
+#pragma unroll
+    for (int k = 0; k < STEPS; k++) {
+        const int r = r0 + k * (THREADS / ACROSS);
+        if (C * ACROSS % THREADS && r >= C) break;
+        const bool row = r >= first && r < end;
+        const T *from = src + r * stride + c;
+        if (wide) {
+            const bool there = row && c < cols;
+            copy_async<sizeof(Piece<T>)>(to + k * THREADS * sizeof(Piece<T>), there ? from : safe, there);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const bool there = row && c + i < cols;
+                if constexpr (sizeof(T) == 4)
+                    copy_async<4>(to + k * THREADS * sizeof(Piece<T>) + 4 * i, there ? from + i : safe, there);
+                else
+                    reinterpret_cast<Piece<T> *>(raw)[threadIdx.x + k * THREADS].v[i] = there ? from[i] : from_float<T>(0.f);
+            }
+        }
+    }
+}
+// TERMS 0: not wanted.  weight: the rows times their weights as a second tile of three terms, and whether this thread met
+// an infinity or NaN, whose first term is itself.
+template <typename T, int TERMS, int C, int COLS, int THREADS, bool WEIGHTED>
+__device__ __forceinline__ bool convert(unsigned char *dst, unsigned char *weighted, const float *weight, const unsigned char *raw) {
+    using L = Tile<C, COLS>;
+    constexpr int ACROSS = COLS / 4, STEPS = (C * ACROSS + THREADS - 1) / THREADS;
+    const int r0 = threadIdx.x / ACROSS, at0 = r0 * L::pitch + threadIdx.x % ACROSS * 8;
+    bool odd = false;
+#pragma unroll
+    for (int k = 0; k < STEPS; k++) {
+        const int step = k * (THREADS / ACROSS);
+        if (C * ACROSS % THREADS && r0 + step >= C) break;
+        const Piece<T> piece = reinterpret_cast<const Piece<T> *>(raw)[threadIdx.x + k * THREADS];
+        float f[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) f[i] = to_float(piece.v[i]);
+        unsigned char *const at = dst + at0 + step * L::pitch;
+        put4<TERMS>(at, L::plane, f[0], f[1], f[2], f[3]);
+        if (!WEIGHTED) continue;
+        const float w = weight[r0 + step];
+        put4<3>(weighted + at0 + step * L::pitch, L::plane, f[0] * w, f[1] * w, f[2] * w, f[3] * w);
+        if (TERMS && !(fabsf(f[0]) + fabsf(f[1]) + fabsf(f[2]) + fabsf(f[3]) <= 3.4e38f)) {
+            odd = true;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (!(fabsf(f[i]) <= 3.4e38f))
+                    for (int j = 1; j < TERMS; j++) *reinterpret_cast<uint16_t *>(at + 2 * i + j * L::plane) = 0;
+        }
+    }
+    return odd;
+}
+
+// SUM: only the segment's own sum of the state, into the workspace.
+template <typename T, int DK, bool SUM>
+__global__ void __launch_bounds__(BlockShape<T, DK, SUM>::THREADS, SUM ? 2 : 1) block_kernel(const __grid_constant__ Passes all) {
+    using L = BlockShape<T, DK, SUM>;
+    constexpr int C = L::C, SLICE = L::SLICE, IN = L::IN;
+    constexpr int ROW_TILES = C / 16, ACROSS = L::WARPS / ROW_TILES;
+    constexpr int SCORE_TILES = C / 8 > ACROSS ? C / 8 / ACROSS : 1, OUT_TILES = SLICE / 8 > ACROSS ? SLICE / 8 / ACROSS : 1;
+    constexpr int STATE_ACROSS = L::WARPS / (DK / 16), STATE_TILES = SLICE / 8 / STATE_ACROSS;
+    static_assert(DK / 16 <= L::WARPS, "a warp keeps 16 rows of the state");
+    extern __shared__ __align__(16) unsigned char shared[];
+    float *const pw = reinterpret_cast<float *>(shared + L::pw), *const weight = reinterpret_cast<float *>(shared + L::weight);
+    const uint32_t base = shared_address(shared);
+    __shared__ int first_odd;
+
+    const int b = blockIdx.z % (unsigned)all.pass[0].p.batch;
+    const MixPass &cp = all.pass[blockIdx.z / (unsigned)all.pass[0].p.batch];
+    const MixParams &p = cp.p;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int slices = gridDim.y / p.heads;
+    const int segment = blockIdx.x, h = blockIdx.y / slices, c0 = blockIdx.y % slices * SLICE;
+    const int cols = min(SLICE, p.dv - c0);
+    // (the pass after a sum: that has waited for the inputs)
+    if (SUM || cp.count == 1) wait_for_previous();
+    const Line line(cp, segment, h, b);
+    if (!SUM && (segment > line.last || c0 >= p.dv)) wait_for_previous();
+    if (SUM) let_next_start();
+    if (c0 >= p.dv) return;  // the widest pass decides the grid
+    if (segment > line.last || (SUM && ((segment == line.last && !p.s_out) || line.count == 0))) return;
+    const int chunks = (line.tokens + C - 1) / C;  // none for an empty sequence, whose state passes through
+    const float log_decay = p.log_decay[h];
+    for (int i = tid; i <= C; i += L::THREADS) pw[i] = i ? (float)exp((double)log_decay * i) : 1.f;
+
+    // this warp's part of the state: rows state_row + g, + 8, columns state_col + 8 n + 2 t, + 1
+    const int state_row = warp / STATE_ACROSS * 16, state_col = warp % STATE_ACROSS * STATE_TILES * 8;
+    float s[STATE_TILES][4];
+    float *const own = segment_state(cp, b, h, segment);
+    if (!SUM && cp.count > 1) wait_for_previous();
+    if (!SUM) let_next_start();
+    const float *in = SUM ? nullptr : cp.count > 1 ? own : p.s_in && line.kept ? p.s_in + line.user : nullptr;
+    float *out = SUM ? own : cp.count == 1 && p.s_out && line.kept ? p.s_out + line.user : nullptr;
+    const int64_t in_k = cp.count > 1 ? p.dv : p.state_k, in_v = cp.count > 1 ? 1 : p.state_v;  // of `out` too
+#pragma unroll
+    for (int n = 0; n < STATE_TILES; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int r = state_row + g + (e >> 1) * 8, c = state_col + 8 * n + 2 * t + (e & 1);
+            s[n][e] = in && r < p.dk && c < cols ? in[r * in_k + (c0 + c) * in_v] : 0.f;
+        }
+    auto publish_state = [&] {
+#pragma unroll
+        for (int n = 0; n < STATE_TILES; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e += 2)
+                put<3>(shared + L::s + (state_row + g + e * 4) * L::State::pitch + (state_col + 8 * n + 2 * t) * 2, L::State::plane,
+                       s[n][e], s[n][e + 1]);
+    };
+
+    const T *q = static_cast<const T *>(p.q.p) + (p.offsets ? 0 : b * p.q.sb) + (h / p.q.per_head) * p.q.sh;
+    const T *k = static_cast<const T *>(p.k.p) + (p.offsets ? 0 : b * p.k.sb) + (h / p.k.per_head) * p.k.sh;
+    const T *v = static_cast<const T *>(p.v.p) + (p.offsets ? 0 : b * p.v.sb) + (h / p.v.per_head) * p.v.sh + c0;
+    const int64_t out_at = (p.offsets ? 0 : b * p.osb) + h * p.osh + c0;
+    auto write = [&](int64_t row, int col, float y) {
+        if (cp.out_f32)
+            static_cast<float *>(p.o)[out_at + row * p.ost + col] = y;
+        else
+            static_cast<T *>(p.o)[out_at + row * p.ost + col] = from_float<T>(y);
+    };
+    const int out_bytes = cp.out_f32 ? 4 : sizeof(T);
+    const bool pairs = cols % 2 == 0 && p.ost % 2 == 0 && (reinterpret_cast<uintptr_t>(p.o) + out_at * out_bytes) % (2 * out_bytes) == 0;
+    auto write_two = [&](int64_t row, int col, float a, float b) {
+        if (col >= cols) return;
+        if (!pairs) {
+            write(row, col, a);
+            if (col + 1 < cols) write(row, col + 1, b);
+        } else if (sizeof(T) == 4 || cp.out_f32) {
+            *reinterpret_cast<float2 *>(static_cast<float *>(p.o) + out_at + row * p.ost + col) = {a, b};
+        } else {
+            if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t *>(static_cast<T *>(p.o) + out_at + row * p.ost + col) = pack<T>(a, b);
+        }
+    };
+    const int row0 = warp / ACROSS * 16;  // of the chunk, for scores and results
+    const int score_col = warp % ACROSS * SCORE_TILES * 8, out_col = warp % ACROSS * OUT_TILES * 8;
+    const float inside = p.update * p.out;
+    int powers_of = 0;
+    Fade keep{1.f, 0.f};
+
+    auto fetch_chunk = [&](int c) {
+        const int at = line.from + c * C, n = min(C, line.tokens - c * C), first = p.reverse ? C - n : 0;
+        const int64_t start = line.start + (p.reverse ? line.count - at - C : at);
+        fetch<T, C, DK, L::THREADS>(shared + L::raw_k, k + start * p.k.st, p.k.st, first, first + n, p.dk);
+        fetch<T, C, SLICE, L::THREADS>(shared + L::raw_v, v + start * p.v.st, p.v.st, first, first + n, cols);
+        if (!SUM) fetch<T, C, DK, L::THREADS>(shared + L::raw_q, q + start * p.q.st, p.q.st, first, first + n, p.dk);
+    };
+    if (chunks) fetch_chunk(0);
+    for (int c = 0; c < chunks; c++) {
+        const int at = line.from + c * C, n = min(C, line.tokens - c * C);
+        const int first = p.reverse ? C - n : 0, end = first + n;  // valid tile rows
+        const int64_t start = line.start + (p.reverse ? line.count - at - C : at);
+        __syncthreads();  // nobody reads the tiles any more
+        if (n != powers_of) {  // the first chunk, and a last one that is shorter
+            powers_of = n;
+            keep = fade_of((double)log_decay * n);
+            if (tid < C) weight[tid] = tid >= first && tid < end ? p.update * pw[p.reverse ? tid + 1 - first : end - 1 - tid] : 0.f;
+            __syncthreads();
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        convert<T, IN, C, DK, L::THREADS, false>(shared + L::k, nullptr, nullptr, shared + L::raw_k);
+        const bool odd = convert<T, SUM ? 0 : IN, C, SLICE, L::THREADS, true>(shared + L::v, shared + L::w, weight, shared + L::raw_v);
+        if (!SUM) {
+            convert<T, IN, C, DK, L::THREADS, false>(shared + L::q, nullptr, nullptr, shared + L::raw_q);
+            publish_state();
+        }
+        if (c + 1 < chunks) fetch_chunk(c + 1);
+        const bool careful = __syncthreads_or(odd);
+
+        if (!SUM && score_col < C) {
+            float x[SCORE_TILES][4] = {};
+            const bool none = p.reverse ? score_col + SCORE_TILES * 8 <= row0 : score_col >= row0 + 16;
+            if (!none)
+                multiply<IN, IN, SCORE_TILES, false, false>(x, operand_a<false>(base + L::q, L::Keys::pitch, L::Keys::plane, row0),
+                                                            operand_b<false>(base + L::k, L::Keys::pitch, L::Keys::plane, score_col), 0, DK / 16);
+#pragma unroll
+            for (int m = 0; m < SCORE_TILES; m++)
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                    const int i = row0 + g + e * 4, j = score_col + 8 * m + 2 * t, gap = p.reverse ? j - i : i - j,
+                              next = p.reverse ? gap + 1 : gap - 1;
+                    put<3>(shared + L::p + i * L::Scores::pitch + j * 2, L::Scores::plane,
+                           gap >= 0 ? x[m][e] * (inside * pw[max(gap, 0)]) : 0.f,
+                           next >= 0 ? x[m][e + 1] * (inside * pw[max(next, 0)]) : 0.f);
+                }
+        }
+
+        // state
+#pragma unroll
+        for (int j = 0; j < STATE_TILES; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[j][e] = faded(s[j][e], keep);
+        if (state_col < cols)
+            multiply<IN, 3, STATE_TILES, true, true>(s, operand_a<true>(base + L::k, L::Keys::pitch, L::Keys::plane, state_row),
+                                                     operand_b<true>(base + L::w, L::Values::pitch, L::Values::plane, state_col), 0, C / 16);
+        if (SUM) continue;
+        __syncthreads();
+
+        // Infinities and NaN among the values: a masked score of zero times them would spread them to tokens before
+        // them.  The rows from the first of them on are summed one by one; the others' product goes without them.
+        int stop = C;
+        if (careful) {
+            if (tid == 0) first_odd = C;
+            __syncthreads();
+            for (int u = tid; u < C * SLICE; u += L::THREADS)
+                if (!(fabsf(get<IN>(shared + L::v + u / SLICE * L::Values::pitch + u % SLICE * 2, L::Values::plane)) <= 3.4e38f))
+                    atomicMin(&first_odd, p.reverse ? C - 1 - u / SLICE : u / SLICE);
+            __syncthreads();
+            stop = first_odd;
+            for (int u = tid; u < C * SLICE; u += L::THREADS) {
+                const int i = u / SLICE, col = u % SLICE;
+                if (i < first || i >= end || col >= cols || (p.reverse ? C - 1 - i : i) < stop) continue;
+                float state = 0.f, sum = 0.f;
+                for (int d = 0; d < DK; d++)
+                    state = fmaf(get<IN>(shared + L::q + i * L::Keys::pitch + d * 2, L::Keys::plane),
+                                 get<3>(shared + L::s + d * L::State::pitch + col * 2, L::State::plane), state);
+                for (int j = p.reverse ? i : 0; j < (p.reverse ? C : i + 1); j++)
+                    sum = fmaf(get<3>(shared + L::p + i * L::Scores::pitch + j * 2, L::Scores::plane),
+                               get<IN>(shared + L::v + j * L::Values::pitch + col * 2, L::Values::plane), sum);
+                if (p.o) write(start + i, col, fmaf(p.out * pw[p.reverse ? C - 1 - i : i + 1], state, sum));
+            }
+            __syncthreads();
+            for (int u = tid; u < C * SLICE; u += L::THREADS) {
+                unsigned char *f = shared + L::v + u / SLICE * L::Values::pitch + u % SLICE * 2;
+                if (!(fabsf(get<IN>(f, L::Values::plane)) <= 3.4e38f))
+                    for (int i = 0; i < IN; i++) *reinterpret_cast<uint16_t *>(f + i * L::Values::plane) = 0;
+            }
+            __syncthreads();
+        }
+
+        // results: the state's part, faded by row, and the part inside the chunk
+        if (out_col >= cols) continue;  // columns past the last
+        float y[OUT_TILES][4] = {};
+        multiply<IN, 3, OUT_TILES, false, true>(y, operand_a<false>(base + L::q, L::Keys::pitch, L::Keys::plane, row0),
+                                                operand_b<true>(base + L::s, L::State::pitch, L::State::plane, out_col), 0, DK / 16);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int i = row0 + g + (e >> 1) * 8;
+            const float fade = p.out * pw[p.reverse ? C - 1 - i : i + 1];
+#pragma unroll
+            for (int m = 0; m < OUT_TILES; m++) y[m][e] *= fade;
+        }
+        // (only the columns of scores that this row tile has)
+        multiply<3, IN, OUT_TILES, false, true>(y, operand_a<false>(base + L::p, L::Scores::pitch, L::Scores::plane, row0),
+                                                operand_b<true>(base + L::v, L::Values::pitch, L::Values::plane, out_col),
+                                                p.reverse ? row0 / 16 : 0, p.reverse ? C / 16 : row0 / 16 + 1);
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+            const int i = row0 + g + e * 4;
+            if (!p.o || i < first || i >= end || (p.reverse ? C - 1 - i : i) >= stop) continue;
+#pragma unroll
+            for (int m = 0; m < OUT_TILES; m++) write_two(start + i, out_col + 8 * m + 2 * t, y[m][e], y[m][e + 1]);
+        }
+    }
+
+    if (!out) return;
+#pragma unroll
+    for (int j = 0; j < STATE_TILES; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int r = state_row + g + (e >> 1) * 8, col = state_col + 8 * j + 2 * t + (e & 1);
+            if (r < p.dk && col < cols) out[r * in_k + (c0 + col) * in_v] = s[j][e];
+        }
+}
+
+template <typename T, int DK>
+cudaError_t launch_dims(const Passes &all, int passes, cudaStream_t s) {
+    using L = BlockShape<T, DK, false>;
+    const MixPass &first = all.pass[0];
+    int slices = 1;
+    for (int k = 0; k < passes; k++) slices = std::max(slices, (all.pass[k].p.dv + L::SLICE - 1) / L::SLICE);
+    const dim3 grid(first.count, first.p.heads * slices, (unsigned)first.p.batch * passes);
+    if (first.count > 1) {
+        cudaError_t e = launch(block_kernel<T, DK, true>, grid, L::THREADS, BlockShape<T, DK, true>::bytes, s, all);
+        if (e == cudaSuccess) e = launch_enter(all, passes, s);
+        if (e != cudaSuccess) return e;
+    }
+    return launch(block_kernel<T, DK, false>, grid, L::THREADS, L::bytes, s, all);
+}
+
+}  // namespace
+
+bool chunked_split_takes(const MixPass &pass) {
+    const MixParams &p = pass.p;
+    const int64_t tokens = p.offsets ? p.packed_tokens : p.length;
+    if ((int64_t)p.heads * 8 > 65535) return false;  // the grid's second axis: up to eight slices of a head
+    return p.length >= 2 && tokens > 0 && std::max(tokens, p.length) <= int64_t(1) << 30;  // rows are counted in 32 bits
+}
+
+static int shape_of(int dk) { return dk <= 32 ? 32 : dk <= 64 ? 64 : dk <= 128 ? 128 : 256; }
+int chunked_split_shape(const MixPass &pass) { return shape_of(pass.p.dk); }
+
+// One CTA to an SM takes `whole` for a chunk's results, and two of them take 0.7 of that for their sums, or one 0.45.
+double chunked_split_time(int64_t lines, int64_t count, double per, int dk, int dv) {
+    const int shape = shape_of(dk), slice = shape == 32 || shape == 256 ? 32 : 64;
+    const double whole = shape == 32 ? 8 : shape == 64 ? 13 : shape == 128 ? 23.5 : 46;
+    const int64_t ctas = lines * count * ((dv + slice - 1) / slice);
+    const double results = (double)((ctas + kSms - 1) / kSms) * (whole * per + 2);
+    if (count == 1) return results;
+    return results + (ctas <= kSms ? 0.45 : 0.7 * (double)((ctas + 2 * kSms - 1) / (2 * kSms))) * whole * per + 12;
+}
+
+cudaError_t launch_chunked_split(const MixPass *passes, int n, Element e, cudaStream_t s) {
+    Passes all{};
+    for (int k = 0; k < n; k++) all.pass[k] = passes[k];
+    return with_element(e, [&](auto v) {
+        using T = decltype(v);
+        switch (chunked_split_shape(passes[0])) {
+            case 32: return launch_dims<T, 32>(all, n, s);
+            case 64: return launch_dims<T, 64>(all, n, s);
+            case 128: return launch_dims<T, 128>(all, n, s);
+            default: return launch_dims<T, 256>(all, n, s);
+        }
+    });
+}
+
+}  // namespace b200fft

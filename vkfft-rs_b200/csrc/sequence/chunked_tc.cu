@@ -105,41 +105,6 @@ __device__ __forceinline__ float tile_value(const unsigned char *t, int r, int c
     return to_float(*reinterpret_cast<const T *>(t + tile_byte(r, c, rows)));
 }
 
-// Two elements in a register.
-template <typename T>
-struct Two;
-template <>
-struct Two<__nv_bfloat16> {
-    using type = __nv_bfloat162;
-    static constexpr uint32_t exponent = 0x7f807f80u, above = 0x00800080u;  // exponent + above: a sign where it is all ones
-    static __device__ __forceinline__ type of(float a, float b) { return __floats2bfloat162_rn(a, b); }
-    static __device__ __forceinline__ float2 wide(type v) { return __bfloat1622float2(v); }
-};
-template <>
-struct Two<__half> {
-    using type = __half2;
-    static constexpr uint32_t exponent = 0x7c007c00u, above = 0x04000400u;
-    static __device__ __forceinline__ type of(float a, float b) { return __floats2half2_rn(a, b); }
-    static __device__ __forceinline__ float2 wide(type v) { return __half22float2(v); }
-};
-template <typename T>
-__device__ __forceinline__ typename Two<T>::type as_two(uint32_t v) { return *reinterpret_cast<const typename Two<T>::type *>(&v); }
-template <typename P>
-__device__ __forceinline__ uint32_t as_word(P v) { return *reinterpret_cast<const uint32_t *>(&v); }
-template <typename T>
-__device__ __forceinline__ uint32_t pack(float a, float b) { return as_word(Two<T>::of(a, b)); }
-// Two f32 as the sums of three (two) terms each.
-template <typename T, int TERMS>
-__device__ __forceinline__ void split_terms(float a, float b, uint32_t *t, int step) {
-#pragma unroll
-    for (int k = 0; k < TERMS; k++) {
-        t[k * step] = pack<T>(a, b);
-        const float2 w = Two<T>::wide(as_two<T>(t[k * step]));
-        a -= w.x;
-        b -= w.y;
-    }
-}
-
 // The power of two that brings `most` to [2^top, 2^(top+1)), held within 2^-60 and 2^60, and its inverse.
 // `most` is not negative; where it is no number, or infinite, anything goes.
 struct Scale {
@@ -1171,23 +1136,10 @@ cudaError_t launch_type(const TensorPasses &run, int passes, cudaStream_t s) {
 
 }  // namespace
 
-Segments segments_of(int64_t length, int64_t lines) {
-    const int64_t chunks = (length + kChunk - 1) / kChunk;
-    // microseconds: waves of CTAs, each with its start and its chunks.  One segment: 3.5 a chunk (four terms);
-    // more: 3.1 and 1.6 for the pass before it, twice the start, and the kernel between the two.
-    Segments best{1, (int)chunks};
-    double least = 0;
-    for (int64_t want = 1; want <= std::min<int64_t>(chunks, 64); want++) {
-        const int64_t per = (chunks + want - 1) / want, count = (chunks + per - 1) / per;
-        if (count > 1 && lines * count > 8 * kSms) break;
-        const double waves = (double)((lines * count + kSms - 1) / kSms);
-        const double time = count == 1 ? waves * (3.5 * per + 5) : waves * (4.7 * per + 12) + 10;
-        if (want == 1 || time < least) {
-            least = time;
-            best = {(int)count, (int)per};
-        }
-    }
-    return best;
+// Four terms where a sequence is one segment, else two.
+double chunked_tc_time(int64_t lines, int64_t count, int64_t per) {
+    const double waves = (double)((lines * count + kSms - 1) / kSms);
+    return count == 1 ? waves * (3.5 * per + 5) : waves * (4.7 * per + 12) + 10;
 }
 
 int chunked_tc_shape(const MixPass &pass) { return (pass.p.dk > 64 ? 2 : 0) + (pass.p.dv > 64 ? 1 : 0); }

@@ -54,6 +54,41 @@ __device__ __forceinline__ float mul_pair(float a, float b) { return a * b; }
 __device__ __forceinline__ float add_pair(float a, float b) { return a + b; }
 __device__ __forceinline__ float fma_pair(float a, float b, float c) { return fmaf(a, b, c); }
 
+// Two elements in a register.
+template <typename T>
+struct Two;
+template <>
+struct Two<__nv_bfloat16> {
+    using type = __nv_bfloat162;
+    static constexpr uint32_t exponent = 0x7f807f80u, above = 0x00800080u;  // exponent + above: a sign where it is all ones
+    static __device__ __forceinline__ type of(float a, float b) { return __floats2bfloat162_rn(a, b); }
+    static __device__ __forceinline__ float2 wide(type v) { return __bfloat1622float2(v); }
+};
+template <>
+struct Two<__half> {
+    using type = __half2;
+    static constexpr uint32_t exponent = 0x7c007c00u, above = 0x04000400u;
+    static __device__ __forceinline__ type of(float a, float b) { return __floats2half2_rn(a, b); }
+    static __device__ __forceinline__ float2 wide(type v) { return __half22float2(v); }
+};
+template <typename T>
+__device__ __forceinline__ typename Two<T>::type as_two(uint32_t v) { return *reinterpret_cast<const typename Two<T>::type *>(&v); }
+template <typename P>
+__device__ __forceinline__ uint32_t as_word(P v) { return *reinterpret_cast<const uint32_t *>(&v); }
+template <typename T>
+__device__ __forceinline__ uint32_t pack(float a, float b) { return as_word(Two<T>::of(a, b)); }
+// Two f32 as the sums of three (two) terms each.
+template <typename T, int TERMS>
+__device__ __forceinline__ void split_terms(float a, float b, uint32_t *t, int step) {
+#pragma unroll
+    for (int k = 0; k < TERMS; k++) {
+        t[k * step] = pack<T>(a, b);
+        const float2 w = Two<T>::wide(as_two<T>(t[k * step]));
+        a -= w.x;
+        b -= w.y;
+    }
+}
+
 // First row and number of rows of sequence b.  Offsets are data: whatever they hold, the
 // range stays inside the packed rows and no longer than `length`.
 struct Rows {

@@ -7,8 +7,6 @@ namespace b200fft {
 
 namespace {
 
-constexpr int kChunk = 128;  // tokens that segments are counted in
-
 struct Passes {
     MixPass pass[kMostPasses];
 };

@@ -156,7 +156,21 @@ LinearAttention LinearAttention::from_c(const b200fft_linear_attention_config &c
 // The passes of one call run side by side; how a sequence is cut goes by all of them, wanted or not, so that the bits of
 // one gradient do not depend on which others are asked for.
 Segments LinearAttention::segments(int passes) const {
-    return length < 2 ? Segments{1, 1} : segments_of(length, batch * heads * passes);
+    if (length < 2) return {1, 1};
+    const int64_t chunks = (length + kChunk - 1) / kChunk, lines = batch * heads * passes;
+    const bool split = element == Element::F32 || key_dim > 128 || value_dim > 128;
+    Segments best{1, (int)chunks};
+    double least = 0;
+    for (int64_t want = 1; want <= std::min<int64_t>(chunks, 64); want++) {
+        const int64_t per = (chunks + want - 1) / want, count = (chunks + per - 1) / per;
+        if (count > 1 && lines * count > 8 * kSms) break;
+        const double time = split ? chunked_split_time(lines, count, std::min((double)per, (double)length / kChunk), (int)key_dim, (int)value_dim) : chunked_tc_time(lines, count, per);
+        if (want == 1 || time < least) {
+            least = time;
+            best = {(int)count, (int)per};
+        }
+    }
+    return best;
 }
 
 size_t LinearAttention::segment_bytes(int passes) const {
@@ -176,8 +190,8 @@ static void launch_passes(const MixPass *passes, int n, Element e, cudaStream_t 
     Kind kind[kMostPasses];
     int shape[kMostPasses];
     for (int k = 0; k < n; k++) {
-        kind[k] = chunked_tc_takes(passes[k], e) ? TENSOR : chunked_tf32_takes(passes[k]) ? BLOCK : TOKENS;
-        shape[k] = kind[k] == TENSOR ? chunked_tc_shape(passes[k]) : kind[k] == BLOCK ? chunked_tf32_shape(passes[k]) : 0;
+        kind[k] = chunked_tc_takes(passes[k], e) ? TENSOR : chunked_split_takes(passes[k]) ? BLOCK : TOKENS;
+        shape[k] = kind[k] == TENSOR ? chunked_tc_shape(passes[k]) : kind[k] == BLOCK ? chunked_split_shape(passes[k]) : 0;
     }
     bool gone[kMostPasses] = {};
     for (int k = 0; k < n; k++) {
@@ -191,7 +205,7 @@ static void launch_passes(const MixPass *passes, int n, Element e, cudaStream_t 
                 gone[j] = true;
             }
         check(kind[k] == TENSOR  ? launch_chunked_tc(together, m, e, s)
-              : kind[k] == BLOCK ? launch_chunked_tf32(together, m, e, s)
+              : kind[k] == BLOCK ? launch_chunked_split(together, m, e, s)
                                  : launch_recurrent(together[0], e, s),
               "kernel launch");
     }

@@ -124,7 +124,11 @@ struct MixPass {
 };
 constexpr int kMostPasses = 3;
 
-Segments segments_of(int64_t length, int64_t lines);
+constexpr int kChunk = 128;  // tokens that segments are counted in
+// Microseconds that `lines` sequences' heads take, cut into `count` segments of `per` chunks each: waves of CTAs, with
+// their start, and where there is more than one segment the pass that sums them up and the kernel between the two.
+double chunked_tc_time(int64_t lines, int64_t count, int64_t per);
+double chunked_split_time(int64_t lines, int64_t count, double per, int dk, int dv);  // per: of tokens that there are
 
 // Token by token.
 cudaError_t launch_recurrent(const MixPass &pass, Element e, cudaStream_t s);
@@ -133,10 +137,10 @@ cudaError_t launch_recurrent(const MixPass &pass, Element e, cudaStream_t s);
 bool chunked_tc_takes(const MixPass &pass, Element e);
 int chunked_tc_shape(const MixPass &pass);
 cudaError_t launch_chunked_tc(const MixPass *passes, int n, Element e, cudaStream_t s);
-// The same for every type, dimension, stride and address, on tf32 matrix instructions.
-bool chunked_tf32_takes(const MixPass &pass);
-int chunked_tf32_shape(const MixPass &pass);
-cudaError_t launch_chunked_tf32(const MixPass *passes, int n, Element e, cudaStream_t s);
+// The same for every type, dimension, stride and address, in f32 accuracy.
+bool chunked_split_takes(const MixPass &pass);
+int chunked_split_shape(const MixPass &pass);
+cudaError_t launch_chunked_split(const MixPass *passes, int n, Element e, cudaStream_t s);
 
 // dst[.., g, d] = sum over the share query heads of src[token, g * share + j, d], for up to two tensors
 struct ShareTensor {
