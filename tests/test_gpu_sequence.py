@@ -113,6 +113,15 @@ def test_layer_norm_strides_and_addresses(V, ctx, dtype, features, xs, ys, shift
     assert R.rel(db, gb) <= R.norm_tolerance(dtype, rows) * 4
 
 
+@pytest.mark.parametrize("dtype", ["F32", "F16", "BF16"])
+@pytest.mark.parametrize("features,gap,shift", [(2, 2, 2), (66, 0, 0), (130, 2, 2), (257, 0, 0), (258, 2, 6), (546, 0, 2), (1025, 0, 0),
+                                                (1026, 4, 2), (1230, 0, 0), (2050, 2, 2), (4097, 1, 0), (4098, 2, 2), (8190, 0, 2),
+                                                (8194, 2, 2)])
+def test_layer_norm_pairs(V, ctx, dtype, features, gap, shift):
+    """Rows that pairs of elements divide, at addresses that hold pairs but not sixteen bytes, and widths beside those."""
+    test_layer_norm_strides_and_addresses(V, ctx, dtype, features, features + gap, features + 2 * gap, shift)
+
+
 @pytest.mark.parametrize("features", [64, 1023, 4096, 20000])
 def test_layer_norm_optional_tensors_and_in_place(V, ctx, features):
     rows = 37

@@ -25,9 +25,10 @@ __device__ __forceinline__ float block_sum(float v, float *buf) {
 }
 
 // ---- rows in registers ----------------------------------------------------------------
-// A row belongs to TPR threads of a block, each with VPT vectors of VEC elements (16 bytes, or single elements where
-// rows or addresses are not aligned): one read, mean and centred variance from registers, one write.  Bound by HBM;
-// the weight and bias come from L1 after the first row.
+// A row belongs to TPR threads of a block, each with VPT vectors of VEC elements: one read, mean and centred variance from
+// registers, one write.  Bound by HBM; the weight and bias come from L1 after the first row.
+// VEC is 16 bytes where rows and addresses are aligned to that, else two elements where they are to those (26754 x 1230
+// bf16: 51 us, by single elements 118; its gradient 73, and 136), else one; then it is instructions that bind.
 
 // Rows go by once: loads and stores that do not stay in the caches (16384 x 4096 bf16: 54 -> 52 us).
 // The raw 16 bytes (or one element) of a vector, as they wait for their turn.
@@ -48,6 +49,19 @@ struct Raw {
         } else {
             return pair_of(__uint_as_float(word(i) << 16), __uint_as_float(word(i) & 0xffff0000u));
         }
+    }
+};
+template <typename T>
+struct Raw<T, 2> {
+    typename std::conditional<sizeof(T) == 4, uint2, uint32_t>::type w;
+    __device__ __forceinline__ void load(const T *p) { w = __ldcs(reinterpret_cast<const decltype(w) *>(p)); }
+    __device__ __forceinline__ uint64_t pair(int) const {
+        Raw<T, 16 / sizeof(T)> r;
+        if constexpr (sizeof(T) == 4)
+            r.w = {w.x, w.y, 0, 0};
+        else
+            r.w = {w, 0, 0, 0};
+        return r.pair(0);
     }
 };
 template <typename T>
@@ -86,11 +100,13 @@ struct Pairs {
         if constexpr (VEC == 1) {
             *to = from_float<T>(f[0]);
         } else {
-            uint4 w;
+            using Word = typename std::conditional<sizeof(T) * VEC == 16, uint4,
+                                                   typename std::conditional<sizeof(T) * VEC == 8, uint2, uint32_t>::type>::type;
+            Word w;
             T *e = reinterpret_cast<T *>(&w);
 #pragma unroll
             for (int i = 0; i < VEC; i++) e[i] = from_float<T>(f[i]);
-            __stcs(reinterpret_cast<uint4 *>(to), w);
+            __stcs(reinterpret_cast<Word *>(to), w);
         }
     }
 };
@@ -103,6 +119,9 @@ __device__ __forceinline__ void load_parameters(const void *p, Element type, int
         const float *q = static_cast<const float *>(p) + at;
         if constexpr (VEC == 1) {
             f[0] = *q;
+        } else if constexpr (VEC == 2) {
+            const float2 w = *reinterpret_cast<const float2 *>(q);
+            f[0] = w.x, f[1] = w.y;
         } else {
 #pragma unroll
             for (int i = 0; i < VEC; i += 4) {
@@ -115,6 +134,8 @@ __device__ __forceinline__ void load_parameters(const void *p, Element type, int
         uint32_t w[(VEC + 1) / 2];
         if constexpr (VEC == 1) {
             w[0] = *q;
+        } else if constexpr (VEC == 2) {
+            w[0] = *reinterpret_cast<const uint32_t *>(q);
         } else {
 #pragma unroll
             for (int i = 0; i < VEC / 4; i++) {
@@ -239,7 +260,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_kernel(const __gri
 // sums in registers.  Otherwise (rows of 1024 threads, whose 64 registers do not hold that) they stand in shared memory:
 // 8 bytes read and written for each element, half of what the row takes from HBM at HBM's pace.
 template <typename T, int VEC, int TPR, int VPT, bool NEXT>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, VEC == 1 ? 1024 / (TPR < 256 ? 256 : TPR) : TPR <= 256 ? 2 : 1) norm_grad_kernel(const __grid_constant__ NormGradParams p) {
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, VEC == 1 ? 1024 / (TPR < 256 ? 256 : TPR) : TPR <= 256 ? (VEC == 2 ? 3 : 2) : 1) norm_grad_kernel(const __grid_constant__ NormGradParams p) {
     constexpr int BLOCK = TPR < 256 ? 256 : TPR, GROUPS = BLOCK / TPR;
     __shared__ float buf[2][BLOCK / 32 * 2];
     extern __shared__ __align__(16) float columns[];  // [2][VPT][VEC][TPR]
@@ -358,6 +379,9 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, VEC == 1 ? 1024 / (TPR 
             if constexpr (VEC == 1) {
                 p.part_w[to] = a[0];
                 p.part_b[to] = b[0];
+            } else if constexpr (VEC == 2) {
+                *reinterpret_cast<float2 *>(p.part_w + to) = make_float2(a[0], a[1]);
+                *reinterpret_cast<float2 *>(p.part_b + to) = make_float2(b[0], b[1]);
             } else {
 #pragma unroll
                 for (int i = 0; i < VEC; i += 4) {
@@ -591,14 +615,25 @@ __global__ void __launch_bounds__(kReduceThreads) norm_grad_reduce_kernel(const 
 int grid_of(int64_t n, int64_t most) { return (int)(n < most ? n : most); }
 
 template <typename T>
-bool aligned_rows(const void *p, int64_t stride) {
-    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * sizeof(T) % 16 == 0;
+bool aligned_rows(const void *p, int64_t stride, int bytes = 16) {
+    return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0 && stride * sizeof(T) % bytes == 0;
 }
 
 // Threads and vectors for rows of `units` vectors: the fewest threads that keep a row in registers.
-template <typename F>
+template <int VEC, typename F>
 bool with_row_shape(int64_t units, F &&f) {
-    if (units <= 32)
+    if (VEC <= 2 && units > 128) {
+        if (units <= 256)
+            f(Int<32>(), Int<8>());
+        else if (units <= 1024)
+            f(Int<128>(), Int<8>());
+        else if (units <= 2048)
+            f(Int<256>(), Int<8>());
+        else if (units <= 4096)
+            f(Int<512>(), Int<8>());
+        else
+            return false;
+    } else if (units <= 32)
         f(Int<32>(), Int<1>());
     else if (units <= 64)
         f(Int<32>(), Int<2>());
@@ -622,7 +657,7 @@ bool with_row_shape(int64_t units, F &&f) {
 // The same where a thread also keeps its columns' sums: 16 of them at most, and at 1024 threads in shared memory.
 template <int VEC, typename F>
 bool with_grad_shape(int64_t units, F &&f) {
-    constexpr int MORE = VEC == 1 ? 4 : VEC == 4 ? 4 : 2;
+    constexpr int MORE = VEC <= 4 ? 4 : 2;
     if (units <= 32)
         f(Int<32>(), Int<1>(), std::true_type());
     else if (units <= 64)
@@ -646,12 +681,13 @@ int norm_grad_groups(int64_t rows, int64_t features, int vec) {
     int threads = 0;
     const auto shape = [&](auto tpr, auto, auto) { threads = decltype(tpr)::value; };
     const bool kept = vec == 1   ? with_grad_shape<1>(features, shape)
+                      : vec == 2 ? with_grad_shape<2>(features / 2, shape)
                       : vec == 4 ? with_grad_shape<4>(features / 4, shape)
                                  : with_grad_shape<8>(features / 8, shape);
     if (!kept) return (int)std::clamp<int64_t>(rows / 64, 1, 64);
     // as many rows at a time as fill the SMs (512 threads each, 1024 where a thread has four columns at most), but 8 rows
     // or more to a group: its sums cost 8 bytes a column, written and read
-    const int64_t most = (int64_t)kSms * std::max(1, std::min(8, (vec == 1 ? 1024 : 512) / threads));
+    const int64_t most = (int64_t)kSms * std::max(1, std::min(8, (vec == 1 ? 1024 : vec == 2 ? 768 : 512) / threads));
     return (int)std::clamp<int64_t>(rows / 8, 1, most);
 }
 
@@ -663,7 +699,7 @@ cudaError_t launch_norm(const NormParams &args, Element e, Element param, cudaSt
         constexpr int VEC = 16 / sizeof(T);
         cudaError_t started = cudaSuccess;
         const auto in_registers = [&](auto vec) {
-            return with_row_shape(p.features / decltype(vec)::value, [&](auto tpr, auto vpt) {
+            return with_row_shape<decltype(vec)::value>(p.features / decltype(vec)::value, [&](auto tpr, auto vpt) {
                 constexpr int TPR = decltype(tpr)::value, ROWS = TPR < 128 ? 128 / TPR : 1;
                 started = launch(norm_kernel<T, decltype(vec)::value, TPR, decltype(vpt)::value>,
                                  dim3((unsigned)((p.rows + ROWS - 1) / ROWS)), TPR < 128 ? 128 : TPR, 0, s, p);
@@ -672,7 +708,10 @@ cudaError_t launch_norm(const NormParams &args, Element e, Element param, cudaSt
         const bool wide = p.features % VEC == 0 && aligned_rows<T>(p.x, p.xs) && aligned_rows<T>(p.y, p.ys) &&
                           aligned_rows<T>(p.w, 0) && aligned_rows<T>(p.b, 0);
         const bool few = p.rows < (int64_t(1) << 31);  // a launch's CTAs
-        if (!few || !(wide ? in_registers(Int<VEC>()) : in_registers(Int<1>())))
+        const int two = 2 * sizeof(T), two_parameters = 2 * (int)element_bytes(param);
+        const bool even = p.features % 2 == 0 && aligned_rows<T>(p.x, p.xs, two) && aligned_rows<T>(p.y, p.ys, two) &&
+                          aligned_rows<T>(p.w, 0, two_parameters) && aligned_rows<T>(p.b, 0, two_parameters);
+        if (!few || !(wide ? in_registers(Int<VEC>()) : even ? in_registers(Int<2>()) : in_registers(Int<1>())))
             return with_element(param, [&](auto q) {
                 return launch(norm_long_kernel<T, decltype(q)>, dim3(grid_of(p.rows, 1 << 30)), kThreads, 0, s, p);
             });
@@ -689,7 +728,10 @@ cudaError_t launch_norm_grad(const NormGradParams &args, Element e, Element para
         constexpr int VEC = 16 / sizeof(T);
         const bool wide = p.features % VEC == 0 && aligned_rows<T>(p.x, p.xs) && aligned_rows<T>(p.dy, p.ys) &&
                           aligned_rows<T>(p.dx, p.xs) && aligned_rows<T>(p.w, 0);
-        p.partials = norm_grad_groups(p.rows, p.features, wide ? VEC : 1);
+        const int two = 2 * sizeof(T);
+        const bool even = p.features % 2 == 0 && aligned_rows<T>(p.x, p.xs, two) && aligned_rows<T>(p.dy, p.ys, two) &&
+                          aligned_rows<T>(p.dx, p.xs, two) && aligned_rows<T>(p.w, 0, 2 * (int)element_bytes(param));
+        p.partials = norm_grad_groups(p.rows, p.features, wide ? VEC : even ? 2 : 1);
         p.part_b = p.part_w ? p.part_w + (size_t)p.partials * p.features : nullptr;
         cudaError_t started = cudaSuccess;
         const auto in_registers = [&](auto vec) {
@@ -697,7 +739,7 @@ cudaError_t launch_norm_grad(const NormGradParams &args, Element e, Element para
             return with_grad_shape<V>(p.features / V, [&](auto tpr, auto vpt, auto next) {
                 constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value, GROUPS = TPR < 256 ? 256 / TPR : 1;
                 constexpr bool NEXT = decltype(next)::value;
-                if constexpr (V > 1 && TPR >= 128 && NEXT)
+                if constexpr (V == VEC && TPR >= 128 && NEXT)
                     started = launch(norm_grad_ring_kernel<T, TPR, VPT>, dim3(p.partials), TPR, ring_bytes(TPR), s, p);
                 else
                     started = launch(norm_grad_kernel<T, V, TPR, VPT, NEXT>, dim3((p.partials + GROUPS - 1) / GROUPS),
@@ -706,7 +748,7 @@ cudaError_t launch_norm_grad(const NormGradParams &args, Element e, Element para
         };
         return with_element(param, [&](auto q) {
             using P = decltype(q);
-            if (!(wide ? in_registers(Int<VEC>()) : in_registers(Int<1>()))) {
+            if (!(wide ? in_registers(Int<VEC>()) : even ? in_registers(Int<2>()) : in_registers(Int<1>()))) {
                 // the sums first: dx may take the place of dy
                 if (sums)
                     started = launch(norm_grad_columns_kernel<T>, dim3((unsigned)((p.features + 31) / 32), p.partials), kThreads, 0, s, p);

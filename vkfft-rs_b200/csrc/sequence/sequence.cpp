@@ -56,8 +56,8 @@ LayerNorm LayerNorm::from_c(const b200fft_layer_norm_config &c) {
 
 size_t LayerNorm::backward_workspace() const {
     const int vec = (int)(16 / element_bytes(element));
-    const int groups = std::max(norm_grad_groups(rows, features, 1),
-                                features % vec == 0 ? norm_grad_groups(rows, features, vec) : 1);
+    const int groups = std::max({norm_grad_groups(rows, features, 1), features % 2 == 0 ? norm_grad_groups(rows, features, 2) : 1,
+                                 features % vec == 0 ? norm_grad_groups(rows, features, vec) : 1});
     return (size_t)groups * features * 2 * sizeof(float);
 }
 
