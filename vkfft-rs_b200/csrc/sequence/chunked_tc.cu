@@ -18,6 +18,12 @@
 // f16 has the range of neither scores nor states, so what is rounded to f16 is first multiplied
 // by a power of two, undone in f32: P by row, from the row's largest score; S and W's keys by
 // chunk, from their largest element.  Its two W terms hold 22 bits, f32's own rounding.
+//
+// A chunk takes 3.1 us (W of two terms) or 3.5 (of four) and 2.0 in the pass that only sums up segments, of which the
+// shared memory that products, fragments and tiles go through is busy 4000 cycles of 5900; HBM would let 128 x 128
+// bf16 by in 5550 cycles an SM.  One sequence of 65537 tokens x 8 heads x 128 x 128 takes 180 us, 46 % of HBM's rate
+// (segments read keys and values twice); 8192 x 16 heads 65 us, a third (tensor pipe 31 % busy).  State and results by separate warps, side by side, were slower (65 -> 73 us):
+// the chain W - state - results of a chunk stays, and each link has half the warps.
 #include <algorithm>
 
 #include "segments.cuh"
