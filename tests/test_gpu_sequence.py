@@ -116,7 +116,8 @@ def test_layer_norm_strides_and_addresses(V, ctx, dtype, features, xs, ys, shift
 @pytest.mark.parametrize("dtype", ["F32", "F16", "BF16"])
 @pytest.mark.parametrize("features,gap,shift", [(2, 2, 2), (66, 0, 0), (130, 2, 2), (257, 0, 0), (258, 2, 6), (546, 0, 2), (1025, 0, 0),
                                                 (1026, 4, 2), (1230, 0, 0), (2050, 2, 2), (4097, 1, 0), (4098, 2, 2), (8190, 0, 2),
-                                                (8194, 2, 2)])
+                                                (8194, 2, 2), (1537, 0, 0), (2561, 0, 0), (5119, 0, 0), (5121, 1, 0), (6145, 0, 0),
+                                                (10242, 2, 2), (12290, 0, 2), (16386, 0, 2)])
 def test_layer_norm_pairs(V, ctx, dtype, features, gap, shift):
     """Rows that pairs of elements divide, at addresses that hold pairs but not sixteen bytes, and widths beside those."""
     test_layer_norm_strides_and_addresses(V, ctx, dtype, features, features + gap, features + 2 * gap, shift)

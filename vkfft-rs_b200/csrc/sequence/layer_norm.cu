@@ -28,7 +28,7 @@ __device__ __forceinline__ float block_sum(float v, float *buf) {
 // A row belongs to TPR threads of a block, each with VPT vectors of VEC elements: one read, mean and centred variance from
 // registers, one write.  Bound by HBM; the weight and bias come from L1 after the first row.
 // VEC is 16 bytes where rows and addresses are aligned to that, else two elements where they are to those (26754 x 1230
-// bf16: 51 us, by single elements 118; its gradient 73, and 136), else one; then it is instructions that bind.
+// bf16: 45 us, by single elements 118; its gradient 73, and 136), else one; then it is instructions that bind.
 
 // Rows go by once: loads and stores that do not stay in the caches (16384 x 4096 bf16: 54 -> 52 us).
 // The raw 16 bytes (or one element) of a vector, as they wait for their turn.
@@ -231,24 +231,35 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_kernel(const __gri
     s[0] = sum_of(sum);
     row_sums<TPR>(s, buf[1]);
     const float rstd = 1.f / sqrtf(s[0] / (float)p.features + p.epsilon);
+    // (the parameters' type is looked at once for a row, not for each vector: 16384 x 4096 bf16 48.5 -> 46.4 us,
+    // 8192 x 2047 41 -> 29)
+    const auto finish = [&](auto type) {
+        constexpr Element parameter = decltype(type)::value;
 #pragma unroll
-    for (int k = 0; k < VPT; k++)
-        if (at + k * TPR < units) {
+        for (int k = 0; k < VPT; k++)
+            if (at + k * TPR < units) {
 #pragma unroll
-            for (int i = 0; i < N; i++) v[k].p[i] = mul_pair(v[k].p[i], both<Lane<VEC>>(rstd));
-            Pairs<VEC> w;
-            if (p.w) {
-                load_parameters<VEC>(p.w, p.parameter, (at + k * TPR) * VEC, w);
+                for (int i = 0; i < N; i++) v[k].p[i] = mul_pair(v[k].p[i], both<Lane<VEC>>(rstd));
+                Pairs<VEC> w;
+                if (p.w) {
+                    load_parameters<VEC>(p.w, parameter, (at + k * TPR) * VEC, w);
 #pragma unroll
-                for (int i = 0; i < N; i++) v[k].p[i] = mul_pair(v[k].p[i], w.p[i]);
+                    for (int i = 0; i < N; i++) v[k].p[i] = mul_pair(v[k].p[i], w.p[i]);
+                }
+                if (p.b) {
+                    load_parameters<VEC>(p.b, parameter, (at + k * TPR) * VEC, w);
+#pragma unroll
+                    for (int i = 0; i < N; i++) v[k].p[i] = add_pair(v[k].p[i], w.p[i]);
+                }
+                v[k].store(y + (at + k * TPR) * VEC);
             }
-            if (p.b) {
-                load_parameters<VEC>(p.b, p.parameter, (at + k * TPR) * VEC, w);
-#pragma unroll
-                for (int i = 0; i < N; i++) v[k].p[i] = add_pair(v[k].p[i], w.p[i]);
-            }
-            v[k].store(y + (at + k * TPR) * VEC);
-        }
+    };
+    if (p.parameter == Element::F32)
+        finish(std::integral_constant<Element, Element::F32>());
+    else if (p.parameter == Element::F16)
+        finish(std::integral_constant<Element, Element::F16>());
+    else
+        finish(std::integral_constant<Element, Element::BF16>());
     if (at == 0) {
         if (p.mean) p.mean[row] = mean;
         if (p.rstd) p.rstd[row] = rstd;
@@ -620,17 +631,30 @@ bool aligned_rows(const void *p, int64_t stride, int bytes = 16) {
 }
 
 // Threads and vectors for rows of `units` vectors: the fewest threads that keep a row in registers.
+// Narrow vectors go eight or sixteen to a thread.  Wider rows of single elements are read three times by smaller CTAs
+// (8192 x 7001 bf16: 102 us, 118 in registers); pairs gain up to 16 x 512 (4096 x 16002 f16: 136 -> 88).  More threads
+// with fewer vectors leave an SM one row at a time (768 x 8, 4096 x 4099 bf16: 94 us against 36).
 template <int VEC, typename F>
 bool with_row_shape(int64_t units, F &&f) {
     if (VEC <= 2 && units > 128) {
-        if (units <= 256)
+        if (units <= 8 * 32)
             f(Int<32>(), Int<8>());
-        else if (units <= 1024)
+        else if (units <= 8 * 128)
             f(Int<128>(), Int<8>());
-        else if (units <= 2048)
+        else if (units <= 8 * 192)
+            f(Int<192>(), Int<8>());
+        else if (units <= 8 * 256)
             f(Int<256>(), Int<8>());
-        else if (units <= 4096)
+        else if (units <= 8 * 384)
+            f(Int<384>(), Int<8>());
+        else if (units <= 8 * 512)
             f(Int<512>(), Int<8>());
+        else if (units <= 16 * 320)
+            f(Int<320>(), Int<16>());
+        else if (units <= 16 * 384)
+            f(Int<384>(), Int<16>());
+        else if (VEC == 2 && units <= 16 * 512)
+            f(Int<512>(), Int<16>());
         else
             return false;
     } else if (units <= 32)
