@@ -10,9 +10,9 @@
 // A CTA takes up to 64 value columns of one segment of one head of one sequence; the part of the state that a warp
 // updates stays in its registers in f32, and the next chunk's elements come by cp.async while this one is worked on.
 // One CTA to an SM, as large as shared memory holds: with chunks of 32 tokens, two CTAs of 256 threads took 587 us of
-// 2 x 12960 x 8 heads x 64 x 64, where chunks of 64 take 217 (of which 33 is what memory needs).  Bound by instructions
-// around the products (1.9 a cycle; the matrix pipe is busy a third of the time): of 14000 cycles for a chunk of 64
-// tokens by 64 x 64 in f32, taking elements apart was 4100, scores 2800, the state's update 1600, results 4300; warps
+// 2 x 12960 x 8 heads x 64 x 64, where chunks of 64 take 215 (of which 33 is what memory needs).  Bound by instructions
+// around the products (1.9 a cycle; the matrix pipe is busy a third of the time): of 11000 cycles for a chunk of 64
+// tokens by 64 x 64 in f32, taking elements apart is 2700, scores 2500, the state's update 1600, results 2900; warps
 // with tiles of 16 x 32 in place of 16 x 16 (fewer reads, half as many warps) made it 15 % slower.
 #include <algorithm>
 
@@ -331,6 +331,18 @@ __global__ void __launch_bounds__(BlockShape<T, DK, SUM>::THREADS, SUM ? 2 : 1) 
     int powers_of = 0;
     Fade keep{1.f, 0.f};
 
+    // what this thread's scores are multiplied by; 0 where they are masked
+    float decay[SUM ? 1 : SCORE_TILES][4];
+    if (!SUM) {
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < SCORE_TILES; m++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = row0 + g + (e >> 1) * 8, j = score_col + 8 * m + 2 * t + (e & 1), gap = p.reverse ? j - i : i - j;
+                decay[m][e] = gap >= 0 && gap <= C ? inside * pw[gap] : 0.f;
+            }
+    }
     auto fetch_chunk = [&](int c) {
         const int at = line.from + c * C, n = min(C, line.tokens - c * C), first = p.reverse ? C - n : 0;
         const int64_t start = line.start + (p.reverse ? line.count - at - C : at);
@@ -370,11 +382,9 @@ __global__ void __launch_bounds__(BlockShape<T, DK, SUM>::THREADS, SUM ? 2 : 1) 
             for (int m = 0; m < SCORE_TILES; m++)
 #pragma unroll
                 for (int e = 0; e < 4; e += 2) {
-                    const int i = row0 + g + e * 4, j = score_col + 8 * m + 2 * t, gap = p.reverse ? j - i : i - j,
-                              next = p.reverse ? gap + 1 : gap - 1;
-                    put<3>(shared + L::p + i * L::Scores::pitch + j * 2, L::Scores::plane,
-                           gap >= 0 ? x[m][e] * (inside * pw[max(gap, 0)]) : 0.f,
-                           next >= 0 ? x[m][e + 1] * (inside * pw[max(next, 0)]) : 0.f);
+                    const float a = decay[m][e], b = decay[m][e + 1];  // (0 times an infinite score is not 0)
+                    put<3>(shared + L::p + (row0 + g + e * 4) * L::Scores::pitch + (score_col + 8 * m + 2 * t) * 2, L::Scores::plane,
+                           a != 0.f ? x[m][e] * a : 0.f, b != 0.f ? x[m][e + 1] * b : 0.f);
                 }
         }
 
