@@ -472,6 +472,18 @@ def test_attention_neighbours_stay_apart(V, ctx, dtype):
     assert bool(torch.isfinite(s[0]).all()) and bool(torch.isfinite(s[2]).all()) and not bool(torch.isfinite(s[1]).any())
 
 
+@pytest.mark.parametrize("dtype", ["F32", "F16", "BF16"])
+@pytest.mark.parametrize("part", [-1.0, 0.9975, 0.9946])
+def test_attention_lowest_values_stay_behind(V, ctx, dtype, part):
+    """Values at the ends of the type's range do not reach the tokens before them."""
+    c = Case(V, ctx, [150], 2, 2, 64, 96, dtype)
+    clean, _ = c.forward()
+    start = 83
+    c.v[0, start:start + 3, 1, 5:40] = part * torch.finfo(c.v.dtype).max
+    o, _ = c.forward()
+    assert torch.equal(o[0, :start], clean[0, :start]) and torch.equal(o[:, :, 0], clean[:, :, 0])
+
+
 @pytest.mark.parametrize("dtype,big", [("F16", 60.0), ("BF16", 3e4)])
 def test_attention_large_scores(V, ctx, dtype, big):
     """Scores beyond the range of half precision, weighed down by small values again."""

@@ -234,11 +234,12 @@ __device__ __forceinline__ bool convert(unsigned char *dst, unsigned char *weigh
         if (!WEIGHTED) continue;
         const float w = weight[r0 + step];
         put4<3>(weighted + at0 + step * L::pitch, L::plane, f[0] * w, f[1] * w, f[2] * w, f[3] * w);
-        if (TERMS && !(fabsf(f[0]) + fabsf(f[1]) + fabsf(f[2]) + fabsf(f[3]) <= 3.4e38f)) {
+        // (from 3.39e38 on a first term is infinite)
+        if (TERMS && !(fabsf(f[0]) + fabsf(f[1]) + fabsf(f[2]) + fabsf(f[3]) <= 3.38e38f)) {
             odd = true;
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                if (!(fabsf(f[i]) <= 3.4e38f))
+                if (!(fabsf(f[i]) <= 3.38e38f))
                     for (int j = 1; j < TERMS; j++) *reinterpret_cast<uint16_t *>(at + 2 * i + j * L::plane) = 0;
         }
     }
